@@ -260,6 +260,48 @@ int pto_shampoo_graft(void* p, const void* g, void* acc, const void* P, void* bu
                       size_t ws_bytes, void* stream);
 
 /*
+ * Losses of a language model's head, from hidden states and the head's weight
+ * without the logits (the reference has no counterpart: it starts from
+ * gradients). hidden is [rows, d] with row pitch ldh, weight [vocab, d] with
+ * row pitch ldw (both in elements; weight 16-byte aligned), dtype PTO_F32 or
+ * PTO_BF16. With z = hidden·weightᵀ / T and lse = log Σ exp z, a row's loss is
+ *   cross entropy (T = 1), target y, s = label_smoothing:
+ *     lse - (1-s)·z[y] - s·mean(z) + z_loss·lse²;   y == ignore_index: no row;
+ *   distillation, teacher logits t[k] at token ids index[k] (an id below 0 or
+ *   a logit of -inf is no entry, a row without entries is no row), q =
+ *   softmax(t / T): T²·Σ q·(log q - log softmax(z)[index]).
+ * A target at or past vocab makes its row's loss and the gradients NaN.
+ * Rows that are none have loss 0 and gradient 0 whatever their hidden states
+ * hold, and do not count in the mean (of no row: 0).
+ *
+ * Forward (grad_rows NULL): reduction 0 writes loss[rows], 1 (mean) and 2
+ * (sum) loss[1]. lse[rows] and z[rows·k] (k = 1 for cross entropy), if not
+ * NULL, receive what a later backward call needs (in an order and units of
+ * the library's own). dhidden [rows, d] and dweight [vocab, d] (contiguous, of
+ * dtype; with reduction 1 and 2), if not NULL, receive the gradients of loss.
+ * Backward (grad_rows[rows] not NULL, the gradient of each row's loss):
+ * dhidden and dweight, each if not NULL, from the forward call's lse and z.
+ * The logits of at most about chunk_bytes (0: 2 GiB) are in the workspace at
+ * any time: longer inputs go in chunks of rows. Sums are in a fixed order:
+ * equal calls give equal bits.
+ */
+size_t pto_linear_loss_workspace_bytes(int dtype, int64_t rows, int64_t d, int64_t vocab, int64_t k, int64_t ldw,
+                                       double label_smoothing, int backward, int dhidden, int dweight,
+                                       int64_t chunk_bytes);
+int pto_linear_cross_entropy(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, const int64_t* targets,
+                             int dtype, int64_t rows, int64_t d, int64_t vocab, int64_t ignore_index,
+                             double label_smoothing, double z_loss, int reduction, const float* grad_rows, float* loss,
+                             float* lse, float* z, void* dhidden, void* dweight, int64_t chunk_bytes, void* workspace,
+                             size_t ws_bytes, void* stream);
+int pto_linear_distillation(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
+                            const float* teacher_logits, const int64_t* teacher_index, int dtype, int64_t rows,
+                            int64_t d, int64_t vocab, int64_t k, double temperature, int reduction,
+                            const float* grad_rows, float* loss, float* lse, float* z, void* dhidden, void* dweight,
+                            int64_t chunk_bytes, void* workspace, size_t ws_bytes, void* stream);
+/* x[0..n) *= factor[0] (device pointer) in place, nothing read where it is 1. */
+int pto_scale(void* x, int dtype, int64_t n, const float* factor, void* stream);
+
+/*
  * Kernel timing with HIP events. The reference has no counterpart (its
  * StepTimer, pytorch_opt/optim/_common.py:82-98, is host wall-clock). While
  * enabled, every MFMA launch is bracketed by events on its stream;
@@ -267,7 +309,7 @@ int pto_shampoo_graft(void* p, const void* g, void* acc, const void* P, void* bu
  * launch count for one kernel class ("ns5_gram", "ns5_square",
  * "ns5_update", "kron_left", "kron_right", "gram_update", "root_xmi",
  * "root_pow", "root_mk", "apply_left", "apply_right", "rotate_left",
- * "rotate_right").
+ * "rotate_right", "loss_logits", "loss_dhidden", "loss_dweight").
  */
 int pto_prof_enable(int on);
 int pto_prof_reset(void);

@@ -372,6 +372,23 @@ struct HasSkip : std::false_type {};
 template <class E>
 struct HasSkip<E, std::void_t<decltype(std::declval<const E&>().skip(0, false))>> : std::true_type {};
 
+// An epilogue functor may also carry
+//   `bool adjust(GemmArgs& g, int b, int row0, int col0) const`, which may
+//       shorten g.M and g.K (whole rings of K tiles) for the tile, from counts
+//       that only the device knows; false: the tile has no work (the
+//       workgroup exits). Every wave gets the same answer.
+//   `int q_rows() const`: rows of a K-contiguous Q that exist, where N
+//       counts the padded columns of the output (the rest re-read the last).
+template <class E, class = void>
+struct HasAdjust : std::false_type {};
+template <class E>
+struct HasAdjust<E, std::void_t<decltype(std::declval<const E&>().adjust(std::declval<GemmArgs&>(), 0, 0, 0))>>
+    : std::true_type {};
+template <class E, class = void>
+struct HasQRows : std::false_type {};
+template <class E>
+struct HasQRows<E, std::void_t<decltype(std::declval<const E&>().q_rows())>> : std::true_type {};
+
 // The epilogue of a product kernel, for the fragment rows EFM .. EFM +
 // WTE/16 - 1 of one wave's sub-tile at (wr0, wc0) (all of its rows, or with
 // K groups its half; EFM is a constant so that acc stays in registers).
@@ -717,6 +734,11 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_nt_kernel(Args g, Epi epi) {
     decode_tile<UPPER, sizeof(T) == 2>(logical - b * ntile, g.tiles_m, g.tiles_n, ti, tj);
   }
   const int row0 = ti * BM, col0 = tj * BN;
+  if constexpr (HasAdjust<Epi>::value) {
+    if (!epi.adjust(g, b, row0, col0)) return;
+  }
+  int qrows = g.N;
+  if constexpr (HasQRows<Epi>::value) qrows = epi.q_rows();
   // On a diagonal tile of a symmetric product a wave whose sub-tile lies
   // entirely below the diagonal stores nothing (both epilogue passes use
   // positions i <= j only). In the two-group schedules it still issues its
@@ -755,7 +777,7 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_nt_kernel(Args g, Epi epi) {
       s = static_cast<const T*>(g.P) + (int64_t)b * g.sP + (int64_t)gr * g.ldp + chunk * VEC;
       step[q] = kRowBytes;
     } else if (!QN) {
-      const int gr = min(col0 + (r - BM), max(g.N - 1, 0));
+      const int gr = min(col0 + (r - BM), max(qrows - 1, 0));
       s = static_cast<const T*>(g.Q) + (int64_t)b * g.sQ + (int64_t)gr * g.ldq + chunk * VEC;
       step[q] = kRowBytes;
     } else {

@@ -14,7 +14,8 @@ calls it. Op signatures and defaults are the reference's
 statistics), ``two_sided_product`` (SOAP's rotations), ``adamw_step_``
 (the optimizers' shared AdamW fallback) and ``inverse_matrix_root_each``
 (one root per matrix of a stack, the optimizers' per-factor calls) are
-additive.
+additive, and so are the losses of a language model's head,
+``linear_cross_entropy`` and ``linear_distillation``.
 """
 
 from __future__ import annotations
@@ -177,11 +178,54 @@ def gram_update_(F, X, beta=0.0, alpha=1.0, append_ones=False):
     return reference.gram_update_(F, X, beta=beta, alpha=alpha, append_ones=append_ones)
 
 
+def linear_cross_entropy(hidden, weight, targets, ignore_index=-100, label_smoothing=0.0, z_loss=0.0,
+                         reduction="mean"):
+    """(additive) Cross entropy of a language model's head from hidden states
+    [..., d], the head's weight [vocab, d] and target ids [...], without the
+    logits z = hidden·weightᵀ in memory: per row
+
+        lse(z) - (1 - s)·z[target] - s·mean(z) + z_loss·lse(z)²,  s = label_smoothing.
+
+    Rows whose target is ignore_index take no part: loss and gradient 0
+    whatever their hidden states hold, and the mean is over the others (0 if
+    there are none). A target outside the vocabulary makes its row's loss, and
+    the gradients it reaches, NaN. Returns float32 (float64 for float64
+    inputs): a scalar for reduction "mean" and "sum", one loss per row for
+    "none". Differentiable in hidden and weight, once; with "mean" and "sum"
+    the gradients are found in the forward call, in one pass over the logits.
+    The kernels take float32 and bfloat16, both tensors alike (under autocast
+    both are cast), and keep at most HipBackend.LOSS_CHUNK_BYTES of logits at
+    a time."""
+    if _use_native():
+        return _NATIVE.linear_cross_entropy(hidden, weight, targets, int(ignore_index), float(label_smoothing),
+                                            float(z_loss), str(reduction))
+    return reference.linear_cross_entropy(hidden, weight, targets, ignore_index=ignore_index,
+                                          label_smoothing=label_smoothing, z_loss=z_loss, reduction=reduction)
+
+
+def linear_distillation(hidden, weight, teacher_logits, teacher_index, temperature=1.0, reduction="mean"):
+    """(additive) Distillation of a language model's head from a teacher's top
+    logits: teacher_logits [..., k] at token ids teacher_index [..., k], both
+    constants. With q = softmax(teacher_logits / T) over the row's entries and
+    p the student's softmax(hidden·weightᵀ / T) over the vocabulary, a row's
+    loss is T²·Σ q·(log q - log p). An entry with an id below 0 or a logit of
+    -inf is none, and a row without entries takes no part, as an ignored row
+    of linear_cross_entropy, whose other rules (reduction, types, ids outside
+    the vocabulary, memory) hold here too. At most 1024 entries per row on the
+    GPU; equal ids in a row add up."""
+    if _use_native():
+        return _NATIVE.linear_distillation(hidden, weight, teacher_logits, teacher_index, float(temperature),
+                                           str(reduction))
+    return reference.linear_distillation(hidden, weight, teacher_logits, teacher_index, temperature=temperature,
+                                         reduction=reduction)
+
+
 __all__ = ["get_backend", "set_backend", "native_available", "load_native", "inverse_matrix_root",
            "inverse_matrix_root_each",
            "newton_schulz_orthogonalize", "kron_factor_update_", "kron_factor_update_batched_",
            "precond_apply_two_sided",
            "two_sided_product", "gram_update_", "adamw_step_", "muon_momentum_", "muon_update_", "shampoo_graft_",
+           "linear_cross_entropy", "linear_distillation",
            "OpsArgumentError", "reference"]
 
 if os.environ.get("PYTORCH_OPT_NATIVE") == "1":

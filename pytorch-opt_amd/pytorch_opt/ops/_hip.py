@@ -17,7 +17,7 @@ import math
 
 import torch
 
-from . import reference
+from . import _loss, reference
 from .reference import OpsArgumentError, ROOT_METHODS
 
 _DTYPE_CODE = {torch.float32: 0, torch.float64: 1, torch.bfloat16: 2}
@@ -75,6 +75,15 @@ SIGNATURES = {
     "pto_shampoo_graft_workspace_bytes": (_c_size, []),
     "pto_shampoo_graft": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_i64, _c_dbl, _c_dbl, _c_dbl,
                                    _c_dbl, _c_ptr, _c_ptr, _c_size, _c_ptr]),
+    "pto_linear_loss_workspace_bytes": (_c_size, [_c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_dbl, _c_int,
+                                                  _c_int, _c_int, _c_i64]),
+    "pto_linear_cross_entropy": (_c_int, [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_int, _c_i64, _c_i64, _c_i64,
+                                          _c_i64, _c_dbl, _c_dbl, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                                          _c_ptr, _c_i64, _c_ptr, _c_size, _c_ptr]),
+    "pto_linear_distillation": (_c_int, [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_int, _c_i64, _c_i64,
+                                         _c_i64, _c_i64, _c_dbl, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                                         _c_ptr, _c_i64, _c_ptr, _c_size, _c_ptr]),
+    "pto_scale": (_c_int, [_c_ptr, _c_int, _c_i64, _c_ptr, _c_ptr]),
     "pto_prof_enable": (_c_int, [_c_int]),
     "pto_prof_reset": (_c_int, []),
     "pto_prof_query": (_c_int, [ctypes.c_char_p, ctypes.POINTER(_c_dbl), ctypes.POINTER(_c_i64)]),
@@ -484,6 +493,20 @@ class HipBackend:
         self._check(rc, "gram_update_")
         if Fw is not F:
             F.copy_(Fw)
+
+    # the logits of a loss that may be in the workspace at a time
+    LOSS_CHUNK_BYTES = 2 << 30
+
+    def linear_cross_entropy(self, hidden, weight, targets, ignore_index, label_smoothing, z_loss, reduction):
+        if not hidden.is_cuda:
+            return reference.linear_cross_entropy(hidden, weight, targets, ignore_index, label_smoothing, z_loss,
+                                                  reduction)
+        return _loss.cross_entropy(self, hidden, weight, targets, ignore_index, label_smoothing, z_loss, reduction)
+
+    def linear_distillation(self, hidden, weight, teacher_logits, teacher_index, temperature, reduction):
+        if not hidden.is_cuda:
+            return reference.linear_distillation(hidden, weight, teacher_logits, teacher_index, temperature, reduction)
+        return _loss.distillation(self, hidden, weight, teacher_logits, teacher_index, temperature, reduction)
 
     # ------------------------------------------------------------ timing
     def prof_enable(self, on: bool) -> None:

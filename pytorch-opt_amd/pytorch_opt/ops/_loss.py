@@ -1,0 +1,148 @@
+"""Losses of a language model's head through the HIP library, as torch
+autograd functions (pto_linear_cross_entropy, pto_linear_distillation).
+
+With a mean or sum the forward call also returns the gradients of hidden and
+weight, so the backward only multiplies them by the gradient of the loss (in
+place, and not at all where that is 1). They are handed out once; a second
+backward through a retained graph computes them again. With one loss per row
+the forward keeps lse and the targets' logits, and the backward computes the
+gradients under the rows' own.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import reference
+from .reference import OpsArgumentError
+
+_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 2}
+_REDUCTION_CODE = {"none": 0, "mean": 1, "sum": 2}
+MAX_TEACHER = 1024
+
+
+def _ptr(t):
+    return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+def _rows_readable(t):
+    """t as the library reads a matrix: contiguous rows at a pitch."""
+    return t if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
+
+
+class _Call:
+    """One loss: its constants, and the C call that computes parts of it."""
+
+    def __init__(self, backend, what, labels, k, options, reduction):
+        self.backend, self.what, self.labels, self.k = backend, what, labels, k
+        self.options, self.reduction = options, _REDUCTION_CODE[reduction]
+
+    def __call__(self, h, w, loss=None, lse=None, z=None, dh=None, dw=None, grad_rows=None):
+        be, lib = self.backend, self.backend._lib
+        code, (rows, d), vocab = _DTYPE_CODE[h.dtype], h.shape, w.shape[0]
+        ldh = h.stride(0) if rows > 1 else d
+        ldw = w.stride(0) if vocab > 1 else d
+        smoothing = self.options[1] if self.what == "linear_cross_entropy" else 0.0
+        with torch.cuda.device(h.device):
+            nbytes = lib.pto_linear_loss_workspace_bytes(code, rows, d, vocab, self.k, ldw, smoothing,
+                                                         int(grad_rows is not None), int(dh is not None),
+                                                         int(dw is not None), be.LOSS_CHUNK_BYTES)
+            ws = be._workspace(nbytes, h.device)
+            sizes = (code, rows, d, vocab) if self.what == "linear_cross_entropy" else (code, rows, d, vocab, self.k)
+            rc = getattr(lib, "pto_" + self.what)(
+                _ptr(h), ldh, _ptr(w), ldw, *(_ptr(t) for t in self.labels), *sizes, *self.options, self.reduction,
+                _ptr(grad_rows), _ptr(loss), _ptr(lse), _ptr(z), _ptr(dh), _ptr(dw), be.LOSS_CHUNK_BYTES, _ptr(ws),
+                nbytes, be._stream(h.device))
+        be._check(rc, self.what)
+
+    def gradients(self, h, w, needs, **more):
+        dh = torch.empty(h.shape, dtype=h.dtype, device=h.device) if needs[0] else None
+        dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if needs[1] else None
+        self(h, w, dh=dh, dw=dw, **more)
+        return dh, dw
+
+
+class _LinearLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, w, call, needs):
+        ctx.call, ctx.needs, ctx.grads = call, needs, None
+        h, w = _rows_readable(h), _rows_readable(w)
+        if w.data_ptr() % 16:
+            w = w.clone(memory_format=torch.contiguous_format)
+        if call.reduction:
+            loss = torch.empty((), dtype=torch.float32, device=h.device)
+            if any(needs):
+                ctx.grads = call.gradients(h, w, needs, loss=loss)
+                ctx.save_for_backward(h, w)
+            else:
+                call(h, w, loss=loss)
+            return loss
+        loss = torch.empty(h.shape[0], dtype=torch.float32, device=h.device)
+        lse = z = None
+        if any(needs):
+            lse = torch.empty_like(loss)
+            z = torch.empty(h.shape[0] * call.k, dtype=torch.float32, device=h.device)
+            ctx.save_for_backward(h, w, lse, z)
+        call(h, w, loss=loss, lse=lse, z=z)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        call, be = ctx.call, ctx.call.backend
+        grad = grad.to(torch.float32).contiguous()
+        if not call.reduction:
+            h, w, lse, z = ctx.saved_tensors
+            if h.shape[0] == 0:
+                return (*(torch.zeros_like(t) if n else None for t, n in zip((h, w), ctx.needs)), None, None)
+            dh, dw = call.gradients(h, w, ctx.needs, lse=lse, z=z, grad_rows=grad)
+            return dh, dw, None, None
+        grads, ctx.grads = ctx.grads, None
+        if grads is None:
+            h, w = ctx.saved_tensors
+            grads = call.gradients(h, w, ctx.needs, loss=torch.empty_like(grad))
+        for t in grads:
+            if t is not None:
+                with torch.cuda.device(t.device):
+                    rc = be._lib.pto_scale(_ptr(t), _DTYPE_CODE[t.dtype], t.numel(), _ptr(grad), be._stream(t.device))
+                be._check(rc, call.what)
+        return (*grads, None, None)
+
+
+def _apply(call, hidden, weight, shape):
+    if hidden.dtype not in _DTYPE_CODE:
+        raise OpsArgumentError(f"{call.what}: float32 and bfloat16 on the GPU, got {hidden.dtype}")
+    on = torch.is_grad_enabled()
+    needs = (on and hidden.requires_grad, on and weight.requires_grad)
+    loss = _LinearLoss.apply(hidden.reshape(-1, hidden.shape[-1]), weight, call, needs)
+    return loss if call.reduction else loss.reshape(shape)
+
+
+def _autocast(hidden, weight):
+    if torch.is_autocast_enabled("cuda"):
+        to = torch.get_autocast_dtype("cuda")
+        return hidden.to(to), weight.to(to)
+    return hidden, weight
+
+
+def cross_entropy(backend, hidden, weight, targets, ignore_index, label_smoothing, z_loss, reduction):
+    hidden, weight = _autocast(hidden, weight)
+    reference.check_cross_entropy(hidden, weight, targets, label_smoothing, z_loss, reduction)
+    labels = (targets.reshape(-1).to(torch.int64).contiguous(),)
+    call = _Call(backend, "linear_cross_entropy", labels, 1, (ignore_index, label_smoothing, z_loss), reduction)
+    return _apply(call, hidden, weight, targets.shape)
+
+
+def distillation(backend, hidden, weight, teacher_logits, teacher_index, temperature, reduction):
+    hidden, weight = _autocast(hidden, weight)
+    reference.check_distillation(hidden, weight, teacher_logits, teacher_index, temperature, reduction)
+    k = teacher_index.shape[-1]
+    if k > MAX_TEACHER:
+        raise OpsArgumentError(f"linear_distillation: at most {MAX_TEACHER} teacher entries per row, got {k}")
+    labels = (teacher_logits.detach().reshape(-1).to(torch.float32).contiguous(),
+              teacher_index.reshape(-1).to(torch.int64).contiguous())
+    call = _Call(backend, "linear_distillation", labels, k, (temperature,), reduction)
+    return _apply(call, hidden, weight, teacher_index.shape[:-1])

@@ -225,3 +225,109 @@ def gram_update_(F, X, beta=0.0, alpha=1.0, append_ones=False):
     else:
         F.mul_(beta).add_(prod, alpha=alpha)
     return F
+
+
+# ------------------------------------------------ losses of a model's head
+
+REDUCTIONS = ("none", "mean", "sum")
+
+
+def check_linear_loss(what, hidden, weight, reduction, **per_row):
+    """The argument rules that both backends share; per_row: tensors whose
+    leading shape is the rows'."""
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise OpsArgumentError(f"{what}: hidden [..., d] and weight [vocab, d] expected, got "
+                               f"{tuple(hidden.shape)} and {tuple(weight.shape)}")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise OpsArgumentError(f"{what}: weight has no token or no feature")
+    if hidden.dtype != weight.dtype or not hidden.dtype.is_floating_point:
+        raise OpsArgumentError(f"{what}: hidden and weight must share a floating type, got {hidden.dtype} "
+                               f"and {weight.dtype}")
+    if reduction not in REDUCTIONS:
+        raise OpsArgumentError(f"{what}: reduction must be one of {REDUCTIONS}, got {reduction!r}")
+    for name, t in per_row.items():
+        if tuple(t.shape) != tuple(hidden.shape[:-1]):
+            raise OpsArgumentError(f"{what}: {name} does not match the rows of hidden {tuple(hidden.shape[:-1])}")
+    for t in (weight, *per_row.values()):
+        if t.device != hidden.device:
+            raise OpsArgumentError(f"{what}: every tensor must be on {hidden.device}")
+
+
+def check_cross_entropy(hidden, weight, targets, label_smoothing, z_loss, reduction):
+    check_linear_loss("linear_cross_entropy", hidden, weight, reduction, targets=targets)
+    if targets.dtype.is_floating_point or targets.dtype.is_complex or targets.dtype == torch.bool:
+        raise OpsArgumentError(f"linear_cross_entropy: targets must be token ids, got {targets.dtype}")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise OpsArgumentError(f"linear_cross_entropy: label_smoothing must lie in [0, 1], got {label_smoothing}")
+    if not abs(z_loss) < float("inf"):
+        raise OpsArgumentError(f"linear_cross_entropy: z_loss must be finite, got {z_loss}")
+
+
+def check_distillation(hidden, weight, teacher_logits, teacher_index, temperature, reduction):
+    if teacher_logits.shape != teacher_index.shape or teacher_logits.dim() < 1 or teacher_logits.shape[-1] < 1:
+        raise OpsArgumentError(f"linear_distillation: teacher_logits and teacher_index must share a shape [..., k], "
+                               f"got {tuple(teacher_logits.shape)} and {tuple(teacher_index.shape)}")
+    check_linear_loss("linear_distillation", hidden, weight, reduction, teacher_logits=teacher_logits[..., 0],
+                      teacher_index=teacher_index[..., 0])
+    if not teacher_logits.dtype.is_floating_point or teacher_index.dtype.is_floating_point \
+            or teacher_index.dtype.is_complex or teacher_index.dtype == torch.bool:
+        raise OpsArgumentError(f"linear_distillation: teacher_logits must be floating and teacher_index token ids, "
+                               f"got {teacher_logits.dtype} and {teacher_index.dtype}")
+    if not 0.0 < temperature < float("inf"):
+        raise OpsArgumentError(f"linear_distillation: temperature must be positive, got {temperature}")
+
+
+def _kept_logits(hidden, weight, kept, temperature):
+    """z = hidden·weightᵀ / T in float32 or wider; rows that do not count are
+    replaced by zeros first, so that nothing they hold spreads."""
+    wide = torch.promote_types(hidden.dtype, torch.float32)
+    h = torch.where(kept[:, None], hidden.reshape(-1, hidden.shape[-1]).to(wide), torch.zeros((), dtype=wide,
+                                                                                             device=hidden.device))
+    return (h @ weight.to(wide).T) / temperature
+
+
+def _reduced(loss, kept, shape, reduction):
+    loss = torch.where(kept, loss, torch.zeros((), dtype=loss.dtype, device=loss.device))
+    if reduction == "none":
+        return loss.reshape(shape)
+    return loss.sum() / kept.sum().clamp_min(1) if reduction == "mean" else loss.sum()
+
+
+def linear_cross_entropy(hidden, weight, targets, ignore_index=-100, label_smoothing=0.0, z_loss=0.0,
+                         reduction="mean"):
+    """Cross entropy of hidden·weightᵀ with the logits formed (no counterpart
+    in the reference project); see pytorch_opt.ops.linear_cross_entropy."""
+    check_cross_entropy(hidden, weight, targets, label_smoothing, z_loss, reduction)
+    y = targets.reshape(-1).long()
+    kept = y != ignore_index
+    z = _kept_logits(hidden, weight, kept, 1.0)
+    lse = torch.logsumexp(z, 1)
+    there = (y >= 0) & (y < weight.shape[0])
+    zy = z.gather(1, torch.where(there, y, 0)[:, None])[:, 0] * torch.where(kept & ~there, float("nan"), 1.0)
+    loss = lse - (1.0 - label_smoothing) * zy
+    if label_smoothing:
+        loss = loss - label_smoothing * z.mean(1)
+    if z_loss:
+        loss = loss + z_loss * lse.square()
+    return _reduced(loss, kept, targets.shape, reduction)
+
+
+def linear_distillation(hidden, weight, teacher_logits, teacher_index, temperature=1.0, reduction="mean"):
+    """Distillation from a teacher's top logits with the student's formed (no
+    counterpart in the reference project); see
+    pytorch_opt.ops.linear_distillation."""
+    check_distillation(hidden, weight, teacher_logits, teacher_index, temperature, reduction)
+    index = teacher_index.reshape(-1, teacher_index.shape[-1]).long()
+    wide = torch.promote_types(hidden.dtype, torch.float32)
+    t = teacher_logits.detach().reshape(index.shape).to(wide) / temperature
+    there = (index >= 0) & (t != -float("inf"))
+    kept = there.any(1)
+    z = _kept_logits(hidden, weight, kept, temperature)
+    t = t.masked_fill(~there, -float("inf"))
+    logq = torch.log_softmax(torch.where(kept[:, None], t, 0.0), 1)
+    q = torch.where(there, logq.exp(), 0.0)
+    inside = index < weight.shape[0]
+    zk = z.gather(1, torch.where(there & inside, index, 0)) * torch.where(there & ~inside, float("nan"), 1.0)
+    terms = torch.where(there, torch.where(q == 0, 0.0, q * logq) - q * zk, torch.zeros((), dtype=wide, device=z.device))
+    loss = temperature ** 2 * (torch.logsumexp(z, 1) + terms.sum(1))
+    return _reduced(loss, kept, teacher_index.shape[:-1], reduction)
