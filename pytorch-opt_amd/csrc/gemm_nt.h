@@ -389,6 +389,18 @@ struct HasQRows : std::false_type {};
 template <class E>
 struct HasQRows<E, std::void_t<decltype(std::declval<const E&>().q_rows())>> : std::true_type {};
 
+// kDirect: the epilogue takes the accumulators of a wave as they lie,
+//   `direct(acc, lds, g, wr0, wc0, lane)` (lds: the wave's staging slice), for
+//   K-contiguous operands and wave tiles 64 columns wide. The rows of Q then go
+//   to LDS in another order, row 16·f + l of 64 holding column 4·l + f, so that
+//   lane l of 16 has the four neighbours 4·l .. 4·l + 3 of each of its rows in
+//   its four fragments, and a row's 64 columns are one contiguous store of the
+//   16 lanes: no staging.
+template <class E, class = void>
+struct IsDirect : std::false_type {};
+template <class E>
+struct IsDirect<E, std::enable_if_t<E::kDirect>> : std::true_type {};
+
 // The epilogue of a product kernel, for the fragment rows EFM .. EFM +
 // WTE/16 - 1 of one wave's sub-tile at (wr0, wc0) (all of its rows, or with
 // K groups its half; EFM is a constant so that acc stays in registers).
@@ -777,7 +789,9 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_nt_kernel(Args g, Epi epi) {
       s = static_cast<const T*>(g.P) + (int64_t)b * g.sP + (int64_t)gr * g.ldp + chunk * VEC;
       step[q] = kRowBytes;
     } else if (!QN) {
-      const int gr = min(col0 + (r - BM), max(qrows - 1, 0));
+      int qr = r - BM;
+      if constexpr (IsDirect<Epi>::value) qr = (qr & ~63) | ((qr & 15) << 2) | ((qr >> 4) & 3);
+      const int gr = min(col0 + qr, max(qrows - 1, 0));
       s = static_cast<const T*>(g.Q) + (int64_t)b * g.sQ + (int64_t)gr * g.ldq + chunk * VEC;
       step[q] = kRowBytes;
     } else {
@@ -1387,7 +1401,11 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_nt_kernel(Args g, Epi epi) {
 #undef PTO_EXCHANGE
 #undef PTO_SLOT
   }
-  if constexpr (kSplit) {
+  if constexpr (IsDirect<Epi>::value) {
+    static_assert(!QN && !UPPER && KG == 1 && WTN == 64 && FN == 4, "direct epilogue: 64 columns a wave");
+    epi.direct(acc, reinterpret_cast<char*>(stg), g, wr0, wc0, lane);
+    return;
+  } else if constexpr (kSplit) {
     SplitEpi<Epi> se{epi, plain && !kOwnPlain};
     store_rows<MF, Plan, UPPER, 0>(acc, stg, se, g, b, wr0, wc0, diag, lane);
   } else if constexpr (KG == 1) {

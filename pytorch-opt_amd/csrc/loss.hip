@@ -43,12 +43,13 @@ constexpr int kMaxTeach = 1024;  // sparse targets per row
 constexpr int64_t kChunkBytes = int64_t(2) << 30;  // kept logits of a chunk of rows
 constexpr double kLn2 = 0.6931471805599453;
 
-// bf16 inputs: a kept logit is the number of 2^-9 steps (of log2) it lies
-// below its block's maximum, from 65535 down. p is then off by at most 6.8e-4
-// (bf16's rounding of S: up to 3.9e-3) in the bytes that S takes in the end,
-// and 0 stands for exponentials 2^-128 times the block's largest and less,
-// which fp32 does not hold as normal numbers either. fp32 inputs keep fp32.
-constexpr float kStep = 1.f / 512.f;
+// bf16 inputs: a kept logit is how far it lies below its block's maximum, in
+// log2, as a 16-bit fraction of 128 from the top. p is then off by at most
+// 6.8e-4 (bf16's rounding of S: up to 3.9e-3) in the bytes that S takes in the
+// end, and 0 stands for exponentials 2^-128 times the block's largest and
+// less, which fp32 does not hold as normal numbers either. fp32 inputs keep
+// fp32.
+constexpr float kOctaves = 128.f;
 
 // Sparse targets of a row, k per row in the caller's order. id: the token,
 // -1 where there is none, -2 where it is outside the vocabulary; q: its share;
@@ -279,21 +280,23 @@ __device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x
 
 // ------------------------------------------------------------ the logits
 
-// Exchange within eight consecutive lanes (the lanes of one row in a direct
-// run): neighbours, pairs, halves.
+// Exchange within 16 consecutive lanes (the lanes of one row of an
+// accumulator): neighbours, pairs, halves, the rest.
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, true));
 }
-__device__ __forceinline__ float max8(float v) {
-  v = fmaxf(v, dpp<0xB1>(v));   // quad_perm 1 0 3 2
-  v = fmaxf(v, dpp<0x4E>(v));   // quad_perm 2 3 0 1
-  return fmaxf(v, dpp<0x141>(v));  // row_half_mirror
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, dpp<0xB1>(v));      // quad_perm 1 0 3 2
+  v = fmaxf(v, dpp<0x4E>(v));      // quad_perm 2 3 0 1
+  v = fmaxf(v, dpp<0x141>(v));     // row_half_mirror
+  return fmaxf(v, dpp<0x140>(v));  // row_mirror
 }
-__device__ __forceinline__ float sum8(float v) {
+__device__ __forceinline__ float sum16(float v) {
   v += dpp<0xB1>(v);
   v += dpp<0x4E>(v);
-  return v + dpp<0x141>(v);
+  v += dpp<0x141>(v);
+  return v + dpp<0x140>(v);
 }
 
 // What a row's slopes need besides its logits: S = pa·2^(t − lse2) + pu.
@@ -301,12 +304,13 @@ struct RowSlope {
   float lse2, pa, pu;
 };
 
-// Epilogue of the logits' product. In store_rows a row's 64 columns sit in
-// eight consecutive lanes, eight each; the product's width is padded, so the
-// eight take part together.
+// Epilogue of the logits' product, from the accumulators (kDirect): 16 lanes
+// have a row's 64 columns, four each. Through LDS staging in runs of eight the
+// same work took 14 us of a 256² tile's 69 at d = 2048, most of it VALU.
 template <typename T, bool KEEP, bool SLOPE>
 struct EpiLogits {
   typedef float S;
+  static constexpr bool kDirect = true;
   Chunk ch;
   int vocab;
   float scale;     // log2(e)/T
@@ -316,64 +320,97 @@ struct EpiLogits {
   void* kept;      // KEEP: the kept logits (uint16_t or float); SLOPE: S
   int64_t ld;
   const RowSlope* row;
-  struct Pre {
-    RowSlope r;
-  };
-  typedef NoPre PreT;
-  static constexpr bool kVoIsV = true;
-  __device__ __forceinline__ bool has_t() const { return false; }
   __device__ __forceinline__ bool adjust(GemmArgs& g, int, int row0, int) const {
     g.M = SLOPE ? ch.padded() : ch.live();
     return row0 < g.M;
   }
   __device__ __forceinline__ int q_rows() const { return vocab; }
-  __device__ __forceinline__ void load(int, int i, int, int, int, Pre& p) const {
-    if (SLOPE) p.r = row[i];
-  }
-  __device__ __forceinline__ void load_t(int, int, int, int, PreT&) const {}
-  __device__ __forceinline__ void put_t(int, int, int, const S*, int, const PreT&) const {}
   __device__ __forceinline__ void finish(int) const {}
-  __device__ __forceinline__ void put(int, int i, int j0, const S* v, int, int, const Pre& p, S*) const {
-    float t[8];
+  template <class V, int FM, int FN>
+  __device__ __forceinline__ void direct(const V (&acc)[FM][FN], char* lds, const GemmArgs& g, int wr0, int wc0,
+                                         int lane) const {
+    if (wc0 >= g.N || wr0 >= g.M) return;
+    const int l = lane & 15, sub = (lane >> 4) * 4, c0 = wc0 + 4 * l;
+    const bool whole = wc0 + kCols <= vocab;  // false in the last block of a row at most
+    RowSlope* const rs = reinterpret_cast<RowSlope*>(lds);
     if (SLOPE) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        t[k] = j0 + k < vocab ? fmaf(p.r.pa, pow2(v[k] * scale - p.r.lse2), p.r.pu) : 0.f;
-      st8<T, float>(static_cast<T*>(kept) + i * ld + j0, t, 0, 8);
-      return;
+      for (int r = lane; r < FM * 16; r += 64)
+        if (wr0 + r < g.M) rs[r] = row[wr0 + r];
+      __builtin_amdgcn_s_waitcnt(PTO_LGKM0);
+      __builtin_amdgcn_wave_barrier();
     }
-    float m = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      t[k] = j0 + k < vocab ? v[k] * scale : -INFINITY;
-      m = fmaxf(m, t[k]);
-    }
-    m = max8(m);
-    const float ref = m == -INFINITY ? 0.f : m;  // a block of nothing but -inf sums to 0
-    float s = 0.f;
+    for (int fm = 0; fm < FM; ++fm) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s += pow2(t[k] - ref);
-    s = sum8(s);
-    const int64_t at = i * blocks + j0 / kCols;
-    if (j0 % kCols == 0) stats[at] = make_float2(ref, s);
-    if (sums) {
-      float z = 0.f;
+      for (int r = 0; r < 4; ++r) {
+        const int i = wr0 + fm * 16 + sub + r;
+        const bool live = i < g.M;
+        float v[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) z += j0 + k < vocab ? t[k] : 0.f;
-      z = sum8(z);
-      if (j0 % kCols == 0) sums[at] = z;
-    }
-    if (KEEP) {
-      if constexpr (sizeof(T) == 2) {
-        unsigned u[8];
+        for (int k = 0; k < 4; ++k) v[k] = acc[fm][k][r];
+        if (SLOPE) {
+          const RowSlope p = rs[fm * 16 + sub + r];
+          float t[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) u[k] = (unsigned)fmaxf(fmaf(t[k] - ref, 1.f / kStep, 65535.5f), 0.f);
-        st16(static_cast<uint16_t*>(kept) + i * ld + j0,
-             make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16));
-      } else {
-        st8<float, float>(static_cast<float*>(kept) + i * ld + j0, t, 0, 8);
+          for (int k = 0; k < 4; ++k) t[k] = fmaf(p.pa, pow2(fmaf(v[k], scale, -p.lse2)), p.pu);
+          if (!whole) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) t[k] = c0 + k < vocab ? t[k] : 0.f;
+          }
+          if (live) st4(static_cast<T*>(kept) + i * ld + c0, t);
+          continue;
+        }
+        if (!whole) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = c0 + k < vocab ? v[k] : -INFINITY;
+        }
+        const float m = max16(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+        const float ref = m == -INFINITY ? 0.f : m * scale;  // a block of nothing but -inf sums to 0
+        float x[4], s = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[k] = fmaf(v[k], scale, -ref);
+          s += pow2(x[k]);
+        }
+        s = sum16(s);
+        if (live && l == 0) stats[i * blocks + wc0 / kCols] = make_float2(ref, s);
+        if (sums) {
+          float z = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) z += c0 + k < vocab ? v[k] : 0.f;
+          z = sum16(z) * scale;
+          if (live && l == 0) sums[i * blocks + wc0 / kCols] = z;
+        }
+        if (KEEP && live) {
+          if constexpr (sizeof(T) == 2) {
+            uint2 u;
+            u.x = encode(x[0], x[1]);
+            u.y = encode(x[2], x[3]);
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(kept) + i * ld + c0) = u;
+          } else {
+            float t[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) t[k] = v[k] * scale;
+            st4(static_cast<float*>(kept) + i * ld + c0, t);
+          }
+        }
       }
     }
+  }
+  // (x/128 + 1)·65535, rounded, between 0 and 65535
+  __device__ __forceinline__ static unsigned encode(float a, float b) {
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(fmaf(a, 1.f / kOctaves, 1.f),
+                                                                        fmaf(b, 1.f / kOctaves, 1.f)));
+  }
+  template <typename U>
+  __device__ __forceinline__ static void st4(U* p, const float (&t)[4]) {
+    struct __attribute__((aligned(4 * sizeof(U)))) Run {
+      U e[4];
+    };
+    Run u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) u.e[k] = convert<U>(t[k]);
+    *reinterpret_cast<Run*>(p) = u;
   }
 };
 
@@ -475,11 +512,11 @@ __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __r
       if constexpr (sizeof(T) == 2) {
         const uint4 u = *reinterpret_cast<const uint4*>(static_cast<uint16_t*>(kept) + i * ld + c);
         const unsigned uw[4] = {u.x, u.y, u.z, u.w};
-        const float off = st[c / kCols].x - rs.lse2 - 65535.f * kStep;
+        const float off = st[c / kCols].x - rs.lse2 - kOctaves;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const unsigned x = e & 1 ? uw[e / 2] >> 16 : uw[e / 2] & 0xffffu;
-          const float p = x ? pow2(fmaf((float)x, kStep, off)) : 0.f;
+          const float p = x ? pow2(fmaf((float)x, kOctaves / 65535.f, off)) : 0.f;
           o[e] = c + e < vocab ? fmaf(rs.pa, p, rs.pu) : 0.f;
         }
         uint4 r;
@@ -785,8 +822,11 @@ int launch_nt(const GemmArgs& g, const Epi& e, int batch, bool big, hipStream_t 
   PTO_REQUIRE(g.K % ring_k<T>() == 0 && g.ldp % (16 / sizeof(T)) == 0 && g.ldq % (16 / sizeof(T)) == 0 &&
                   ((reinterpret_cast<uintptr_t>(g.P) | reinterpret_cast<uintptr_t>(g.Q)) & 15) == 0,
               std::string(name) + ": operands not padded or not 16-byte aligned");
-  if (big) return launch_gemm_cfg<T, typename TileSet<T>::big, false>(g, e, batch, s, name);
-  return launch_gemm_cfg<T, typename TileSet<T>::small, false>(g, e, batch, s, name);
+  // a direct epilogue needs 64-column wave tiles: fp32's 128² tile, either bf16 tile
+  if (big || (IsDirect<Epi>::value && sizeof(T) == 4))
+    return launch_gemm_cfg<T, typename TileSet<T>::big, false>(g, e, batch, s, name);
+  if constexpr (!IsDirect<Epi>::value || sizeof(T) == 2) return launch_gemm_cfg<T, typename TileSet<T>::small, false>(g, e, batch, s, name);
+  return -1;
 }
 
 template <typename T>
@@ -841,8 +881,7 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
                          c.ldh, c.d, w.hc, w.dp, static_cast<T*>(c.dh));
       PTO_LAUNCHED("gather");
       GemmArgs g{w.hc, w.dp, 0, W, ldw, 0, ch.cap, (int)w.vp, (int)w.dp, 0, 0, nullptr};
-      // fp32 statistics need 64-column wave tiles: the 128² tile
-      const bool big = f32 || pick_tile<T, false>(ch.cap, w.vp, 1) == 1;
+      const bool big = pick_tile<T, false>(ch.cap, w.vp, 1) == 1;
       if (c.grad_rows) {
         hipLaunchKernelGGL(row_slopes_kernel, dim3((unsigned)((capp + 255) / 256)), dim3(256), 0, s, ch, sp, w.t, z,
                            lse, c.grad_rows, w.slopes);
