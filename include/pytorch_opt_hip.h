@@ -275,28 +275,27 @@ int pto_shampoo_graft(void* p, const void* g, void* acc, const void* P, void* bu
  * hold, and do not count in the mean (of no row: 0).
  *
  * Forward (grad_rows NULL): reduction 0 writes loss[rows], 1 (mean) and 2
- * (sum) loss[1]. lse[rows] and z[rows·k] (k = 1 for cross entropy), if not
+ * (sum) loss[1]. norm[2·rows] and z[rows·k] (k = 1 for cross entropy), if not
  * NULL, receive what a later backward call needs (in an order and units of
  * the library's own). dhidden [rows, d] and dweight [vocab, d] (contiguous, of
  * dtype; with reduction 1 and 2), if not NULL, receive the gradients of loss.
  * Backward (grad_rows[rows] not NULL, the gradient of each row's loss):
- * dhidden and dweight, each if not NULL, from the forward call's lse and z.
+ * dhidden and dweight, each if not NULL, from the forward call's norm and z.
  * The logits of at most about chunk_bytes (0: 2 GiB) are in the workspace at
  * any time: longer inputs go in chunks of rows. Sums are in a fixed order:
  * equal calls give equal bits.
  */
 size_t pto_linear_loss_workspace_bytes(int dtype, int64_t rows, int64_t d, int64_t vocab, int64_t k, int64_t ldw,
-                                       double label_smoothing, int backward, int dhidden, int dweight,
-                                       int64_t chunk_bytes);
+                                       double label_smoothing, int distillation, int backward, int dhidden, int dweight, int64_t chunk_bytes);
 int pto_linear_cross_entropy(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, const int64_t* targets,
                              int dtype, int64_t rows, int64_t d, int64_t vocab, int64_t ignore_index,
                              double label_smoothing, double z_loss, int reduction, const float* grad_rows, float* loss,
-                             float* lse, float* z, void* dhidden, void* dweight, int64_t chunk_bytes, void* workspace,
+                             float* norm, float* z, void* dhidden, void* dweight, int64_t chunk_bytes, void* workspace,
                              size_t ws_bytes, void* stream);
 int pto_linear_distillation(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                             const float* teacher_logits, const int64_t* teacher_index, int dtype, int64_t rows,
                             int64_t d, int64_t vocab, int64_t k, double temperature, int reduction,
-                            const float* grad_rows, float* loss, float* lse, float* z, void* dhidden, void* dweight,
+                            const float* grad_rows, float* loss, float* norm, float* z, void* dhidden, void* dweight,
                             int64_t chunk_bytes, void* workspace, size_t ws_bytes, void* stream);
 /* x[0..n) *= factor[0] (device pointer) in place, nothing read where it is 1. */
 int pto_scale(void* x, int dtype, int64_t n, const float* factor, void* stream);

@@ -17,29 +17,35 @@
 // lists the rows that count, and everything after it works on that list, whose
 // length only the device knows. Then, for chunks of rows:
 //   gather   the chunk's rows of H, padded, and zero rows of dH for left-out ones;
-//   dots     z at the sparse targets, in fp32 (a dot product each);
 //   logits   one MFMA product, whose epilogue takes the maximum and the sum of
-//            exponentials of each row's 64 columns, and for gradients keeps the
-//            block's logits in the workspace;
-//   finish   joins a row's blocks to lse, gives its loss and turns the kept
-//            logits into S;
+//            exponentials of each row's 64 columns and the targets' logits, and
+//            for gradients keeps the block's logits in the workspace;
+//   finish   joins a row's blocks to its normaliser, gives its loss and turns
+//            the kept logits into S;
 //   dH, dW   two MFMA products (dW summed over the chunks in fp32).
 // A pass over V·rows logits is 2·rows·d·V operations, the three products
 // 6·rows·d·V: gradients found in the forward call need no second pass over the
 // logits (8·rows·d·V). Where the rows' gradients come later (losses per row),
-// lse and the targets' z are kept and the backward call forms S in the logits'
-// epilogue.
+// the normaliser and the targets' logits are kept and the backward call forms S
+// in the logits' epilogue.
+//
+// A target's logit is the one that entered the sum of exponentials, so that
+// what it is off by cancels in lse − z_y and p − 1 where p is near 1 (with a
+// separate dot product a loss of 0.1 was off by 1e-5). For the same reason lse
+// is kept as the largest logit m and s = Σ exp(z − m): p = exp(z − m)/s.
 #include <algorithm>
 #include <cmath>
 
 #include "aux_kernels.h"
 #include "gemm_nt.h"
+#include "split.h"
 
 namespace pto {
 namespace {
 
 constexpr int kCols = 64;      // columns of a row that one entry of the statistics covers
 constexpr int kMaxTeach = 1024;  // sparse targets per row
+constexpr int64_t kMaxMarked = 393216;  // tokens whose marks (10 bytes per 64) fit in 64 KB of LDS
 constexpr int64_t kChunkBytes = int64_t(2) << 30;  // kept logits of a chunk of rows
 constexpr double kLn2 = 0.6931471805599453;
 
@@ -51,29 +57,35 @@ constexpr double kLn2 = 0.6931471805599453;
 // fp32.
 constexpr float kOctaves = 128.f;
 
-// Sparse targets of a row, k per row in the caller's order. id: the token,
-// -1 where there is none, -2 where it is outside the vocabulary; q: its share;
-// put: what of S to take off at id (the first of equal ids has their sum, the
-// others -1: nothing to do).
+// Sparse targets. Cross entropy has one per row, by listed row: the token, or
+// -2 where it is outside the vocabulary, with the same share in every row.
+// Distillation has k per row of the call, in the caller's order: the token, -1
+// where there is none, -2 outside the vocabulary; q its share; put what of S to
+// take off at the token (the first of equal ids has their sum, the others -1:
+// nothing to do); entropy Σ q·log q.
 struct Targets {
+  int* one;
+  float share;
   int* id;
-  float *q, *put;
-  float* entropy;  // per row: Σ q·log q
-  int* kept;       // per row: whether the row counts
+  float *q, *put, *entropy;
+  int* kept;   // per row: whether the row counts
+  // a chunk's tokens as a bit set, by 64 columns and row ([blocks][cap]), with
+  // the number of bits in the row before them, and the rank of each entry's
+  // token in its row ([cap][k])
+  unsigned long long* bits;
+  uint16_t* before;
+  uint16_t* rank;
 };
-
-__global__ void __launch_bounds__(256) ce_targets_kernel(const int64_t* __restrict__ y, int64_t rows, int64_t vocab,
-                                                         int64_t ignore, float share, Targets t,
-                                                         float* __restrict__ loss) {
-  const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (r >= rows) return;
-  const int64_t v = y[r];
-  t.kept[r] = v != ignore;
-  t.id[r] = v == ignore ? -1 : v >= 0 && v < vocab ? (int)v : -2;
-  t.q[r] = t.put[r] = share;
-  t.entropy[r] = 0.f;
-  if (loss) loss[r] = 0.f;
-}
+// The targets of one row.
+struct RowTargets {
+  const Targets& t;
+  int64_t at, row;
+  int k;
+  __device__ __forceinline__ int id(int e) const { return t.one ? t.one[at] : t.id[row * k + e]; }
+  __device__ __forceinline__ float q(int e) const { return t.one ? t.share : t.q[row * k + e]; }
+  __device__ __forceinline__ float put(int e) const { return t.one ? t.share : t.put[row * k + e]; }
+  __device__ __forceinline__ float entropy() const { return t.one ? 0.f : t.entropy[row]; }
+};
 
 __device__ __forceinline__ float wave_max(float v) {
   for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
@@ -84,104 +96,113 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
-// One wave per row: the teacher's softmax over the entries that are there
-// (id >= 0, logit above -inf).
+// The teacher's softmax over a row's entries that are there (id >= 0, logit
+// above -inf), one wave per row.
 __global__ void __launch_bounds__(256) kd_targets_kernel(const float* __restrict__ logit,
                                                          const int64_t* __restrict__ index, int64_t rows, int k,
-                                                         int64_t vocab, float inv_temp, Targets t,
-                                                         float* __restrict__ loss) {
-  __shared__ int ids[4][kMaxTeach];
-  __shared__ float qs[4][kMaxTeach];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t r = (int64_t)blockIdx.x * 4 + w;
+                                                         int64_t vocab, float inv_temp, Targets t) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= rows) return;
   const float* lr = logit + r * k;
   const int64_t* ir = index + r * k;
+  constexpr int PER = kMaxTeach / 64;
+  float v[PER];
+  unsigned there = 0;
   float m = -INFINITY;
-  int n = 0;
-  for (int e = lane; e < k; e += 64) {
-    const float v = lr[e] * inv_temp;
+#pragma unroll
+  for (int q = 0; q < PER; ++q) {
+    const int e = q * 64 + lane;
+    v[q] = -INFINITY;
+    if (e >= k) continue;
+    v[q] = lr[e] * inv_temp;
     const int64_t id = ir[e];
-    const bool there = id >= 0 && !(v == -INFINITY);
-    ids[w][e] = !there ? -1 : id < vocab ? (int)id : -2;
-    qs[w][e] = v;
-    if (there) {
-      m = fmaxf(m, v);
-      ++n;
-    }
+    if (id >= 0 && !(v[q] == -INFINITY)) there |= 1u << q;
+    t.id[r * k + e] = !(there >> q & 1) ? -1 : id < vocab ? (int)id : -2;
+    if (there >> q & 1) m = fmaxf(m, v[q]);
   }
   m = wave_max(m);
-  n = __any(n > 0);
   float s = 0.f;
-  for (int e = lane; e < k; e += 64)
-    if (ids[w][e] != -1) s += expf(qs[w][e] - m);
-  s = wave_sum(s);
-  const float logs = logf(s);
+#pragma unroll
+  for (int q = 0; q < PER; ++q)
+    if (there >> q & 1) s += expf(v[q] - m);
+  const float logs = logf(wave_sum(s));
   float ent = 0.f;
-  for (int e = lane; e < k; e += 64) {
-    float q = 0.f;
-    if (ids[w][e] != -1) {
-      const float logq = qs[w][e] - m - logs;
-      q = expf(logq);
-      if (q != 0.f) ent += q * logq;
-    }
-    qs[w][e] = q;
+#pragma unroll
+  for (int q = 0; q < PER; ++q) {
+    const int e = q * 64 + lane;
+    const float logq = v[q] - m - logs, share = there >> q & 1 ? expf(logq) : 0.f;
+    if (share != 0.f) ent += share * logq;
+    if (e < k) t.q[r * k + e] = share;
   }
   ent = wave_sum(ent);
-  __builtin_amdgcn_s_waitcnt(PTO_LGKM0);
-  __builtin_amdgcn_wave_barrier();
-  for (int e = lane; e < k; e += 64) {
-    const int id = ids[w][e];
-    float put = -1.f;
-    if (id >= 0) {
-      put = 0.f;
-      for (int o = 0; o < k; ++o) {
-        if (ids[w][o] != id) continue;
-        if (o < e) {
-          put = -1.f;
-          break;
-        }
-        put += qs[w][o];
-      }
-    }
-    t.id[r * k + e] = id;
-    t.q[r * k + e] = qs[w][e];
-    t.put[r * k + e] = put;
-  }
+  const int any = __any(there != 0);
   if (lane == 0) {
-    t.kept[r] = n;
+    t.kept[r] = any;
     t.entropy[r] = ent;
-    if (loss) loss[r] = 0.f;
   }
 }
 
-// list = the rows that count in order, then the others; count[0] = how many
-// count. One workgroup, each thread a run of rows.
-__global__ void __launch_bounds__(1024) list_rows_kernel(const int* __restrict__ kept, int64_t rows,
-                                                         int* __restrict__ list, int* __restrict__ count) {
-  __shared__ int part[1024];
-  const int t = threadIdx.x;
-  const int64_t per = (rows + 1023) / 1024, r0 = min(rows, t * per), r1 = min(rows, r0 + per);
+// list = the rows that count in order, then the others; count = how many
+// count; losses 0. y: cross entropy's targets (listed to t.one as well), else
+// t.kept says which rows count. weights: alpha = scale times the largest
+// magnitude of those that count (for 16-bit S under rows' gradients: the rows
+// are scaled by a common value in fp32, so that equal gradients cost no
+// rounding); else scale, over the count for the mean. One workgroup of 16
+// waves, each a run of rows, 64 at a time.
+__global__ void __launch_bounds__(1024) list_rows_kernel(const int64_t* __restrict__ y, int64_t ignore, int64_t vocab,
+                                                         Targets t, int64_t rows, int* __restrict__ list,
+                                                         int* __restrict__ count, float* __restrict__ losses,
+                                                         const float* __restrict__ weights, float scale, int mean,
+                                                         float* __restrict__ alpha) {
+  __shared__ int part[16];
+  __shared__ float big[16];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t per = (rows + 1023) / 1024 * 64, r0 = w * per, r1 = min(rows, r0 + per);
+  auto counts = [&](int64_t r) { return r < r1 && (y ? y[r] != ignore : t.kept[r] != 0); };
   int n = 0;
-  for (int64_t r = r0; r < r1; ++r) n += kept[r] != 0;
-  part[t] = n;
+  float m = 0.f;
+#pragma unroll 4
+  for (int64_t b = r0; b < r0 + per; b += 64) {
+    const int64_t r = b + lane;
+    const bool c = counts(r);
+    n += __popcll(__ballot(c));
+    if (weights && c && fabsf(weights[r]) < INFINITY) m = fmaxf(m, fabsf(weights[r]));
+    if (losses && r < r1) losses[r] = 0.f;
+  }
+  m = wave_max(m);
+  if (lane == 0) {
+    part[w] = n;
+    big[w] = m;
+  }
   __syncthreads();
-  for (int o = 1; o < 1024; o <<= 1) {
-    const int add = t >= o ? part[t - o] : 0;
-    __syncthreads();
-    part[t] += add;
-    __syncthreads();
+  int yes = 0, total = 0;
+  for (int o = 0; o < 16; ++o) {
+    if (o < w) yes += part[o];
+    total += part[o];
+    m = fmaxf(m, big[o]);
   }
-  const int total = part[1023];
-  int yes = part[t] - n;
-  int64_t no = total + r0 - yes;
-  for (int64_t r = r0; r < r1; ++r) {
-    if (kept[r] != 0)
-      list[yes++] = (int)r;
-    else
-      list[no++] = (int)r;
+  int64_t no = total + min(rows, r0) - yes;
+#pragma unroll 4
+  for (int64_t b = r0; b < r0 + per; b += 64) {
+    const int64_t r = b + lane;
+    const bool c = counts(r);
+    const unsigned long long mask = __ballot(c), before = (1ull << lane) - 1;
+    const int at = __popcll(mask & before);
+    if (c) {
+      list[yes + at] = (int)r;
+      if (y) t.one[yes + at] = y[r] >= 0 && y[r] < vocab ? (int)y[r] : -2;
+    } else if (r < r1) {
+      list[no + lane - at] = (int)r;
+    }
+    const int here = __popcll(mask);
+    yes += here;
+    no += 64 - here;
   }
-  if (t == 0) count[0] = total;
+  if (threadIdx.x == 0) {
+    count[0] = total;
+    alpha[0] = weights ? (m > 0.f ? scale * m : scale) : mean ? scale / (float)max(total, 1) : scale;
+  }
 }
 
 // The rows of a chunk, as the kernels see them.
@@ -194,6 +215,72 @@ struct Chunk {
   // rows that products reading them along K see: zero rows up to a multiple of kPadK
   __device__ __forceinline__ int padded() const { return (live() + kPadK - 1) / kPadK * kPadK; }
 };
+
+// Distillation: the bit sets, ranks and shares by token of a chunk's rows, one
+// workgroup each. LDS: 10 bytes per 64 tokens.
+__global__ void __launch_bounds__(256) mark_targets_kernel(Chunk ch, int64_t blocks, int k, Targets t) {
+  extern __shared__ unsigned long long word[];
+  uint16_t* const before = reinterpret_cast<uint16_t*>(word + blocks);
+  __shared__ int part[256];
+  __shared__ int entries;
+  const int i = blockIdx.x, tid = threadIdx.x;
+  if (i >= ch.live()) return;
+  const int64_t row = ch.list[ch.base + i];
+  const int* id = t.id + row * k;
+  for (int64_t b = tid; b < blocks; b += 256) word[b] = 0;
+  if (tid == 0) entries = 0;
+  __syncthreads();
+  for (int e = tid; e < k; e += 256) {
+    const int v = id[e];
+    if (v < 0) continue;
+    atomicOr(&word[v >> 6], 1ull << (v & 63));
+    atomicAdd(&entries, 1);
+  }
+  __syncthreads();
+  const int64_t per = (blocks + 255) / 256, b0 = min(blocks, tid * per), b1 = min(blocks, b0 + per);
+  int n = 0;
+  for (int64_t b = b0; b < b1; ++b) n += __popcll(word[b]);
+  part[tid] = n;
+  __syncthreads();
+  for (int o = 1; o < 256; o <<= 1) {
+    const int add = tid >= o ? part[tid - o] : 0;
+    __syncthreads();
+    part[tid] += add;
+    __syncthreads();
+  }
+  int run = part[tid] - n;
+  for (int64_t b = b0; b < b1; ++b) {
+    before[b] = (uint16_t)run;
+    run += __popcll(word[b]);
+  }
+  __syncthreads();
+  if (t.bits)
+    for (int64_t b = tid; b < blocks; b += 256) {
+      t.bits[b * ch.cap + i] = word[b];
+      t.before[b * ch.cap + i] = before[b];
+    }
+  const bool repeats = part[255] != entries;
+  for (int e = tid; e < k; e += 256) {
+    const int v = id[e];
+    float put = -1.f;
+    if (v >= 0) {
+      t.rank[(int64_t)i * k + e] = (uint16_t)(before[v >> 6] + __popcll(word[v >> 6] & ((1ull << (v & 63)) - 1)));
+      put = t.q[row * k + e];
+      if (repeats) {
+        put = 0.f;
+        for (int o = 0; o < k; ++o) {
+          if (id[o] != v) continue;
+          if (o < e) {
+            put = -1.f;
+            break;
+          }
+          put += t.q[row * k + o];
+        }
+      }
+    }
+    t.put[row * k + e] = put;
+  }
+}
 
 // A row of n elements (any alignment) into a padded one, one wave.
 template <typename T>
@@ -213,66 +300,71 @@ __device__ __forceinline__ void copy_row(const T* __restrict__ src, int64_t n, T
   }
 }
 
+// dH of a left-out row.
 template <typename T>
-__global__ void __launch_bounds__(256) gather_kernel(Chunk ch, const T* __restrict__ h, int64_t ldh, int64_t d,
-                                                     T* __restrict__ hc, int64_t ldc, T* __restrict__ dh) {
+__device__ __forceinline__ void zero_row(T* __restrict__ row, int64_t d, int lane) {
+  for (int64_t c = lane; c < d; c += 64) row[c] = T(0.f);
+}
+__global__ void __launch_bounds__(256) gather_kernel(Chunk ch, const bf16* __restrict__ h, int64_t ldh, int64_t d,
+                                                     bf16* __restrict__ hc, int64_t ldc, bf16* __restrict__ dh) {
   const int lane = threadIdx.x & 63;
   const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= ch.padded() && (dh == nullptr || ch.base + i >= ch.rows || i >= ch.cap)) return;
-  if (i < ch.live()) {
+  if (i < ch.live())
     copy_row(h + ch.list[ch.base + i] * ldh, d, hc + i * ldc, ldc, lane);
-    return;
-  }
-  constexpr int E = 16 / (int)sizeof(T);
-  if (i < ch.padded())
-    for (int64_t c = lane * E; c < ldc; c += 64 * E) *reinterpret_cast<uint4*>(hc + i * ldc + c) = make_uint4(0, 0, 0, 0);
-  if (dh && i < ch.cap && ch.base + i < ch.rows) {
-    T* row = dh + ch.list[ch.base + i] * d;
-    for (int64_t c = lane; c < d; c += 64) row[c] = T(0.f);
-  }
+  else if (i < ch.padded())
+    copy_row(h, 0, hc + i * ldc, ldc, lane);
+  if (dh && i >= ch.live() && i < ch.cap) zero_row(dh + ch.list[ch.base + i] * d, d, lane);
 }
 
 // W padded to a multiple of kPadK rows and columns.
-template <typename T>
-__global__ void __launch_bounds__(256) pad_weight_kernel(const T* __restrict__ w, int64_t ldw, int64_t vocab, int64_t d,
-                                                         T* __restrict__ out, int64_t ldo, int64_t rows) {
+__global__ void __launch_bounds__(256) pad_weight_kernel(const bf16* __restrict__ w, int64_t ldw, int64_t vocab,
+                                                         int64_t d, bf16* __restrict__ out, int64_t ldo, int64_t rows) {
   const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= rows) return;
   copy_row(w + min(r, vocab - 1) * ldw, r < vocab ? d : 0, out + r * ldo, ldo, threadIdx.x & 63);
 }
 
-// z at the sparse targets in units of log2 (scale = log2(e)/T), one wave each:
-// out[(base + i)·k + e].
-template <typename T>
-__global__ void __launch_bounds__(256) dots_kernel(Chunk ch, const T* __restrict__ hc, int64_t ldc,
-                                                   const T* __restrict__ w, int64_t ldw, int64_t d, int k, Targets t,
-                                                   float scale, float* __restrict__ out) {
-  constexpr int E = 16 / (int)sizeof(T);
-  const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t i = id / k, e = id % k;
-  if (i >= ch.live()) return;
-  const int v = t.id[(int64_t)ch.list[ch.base + i] * k + e];
-  float s = v == -2 ? NAN : 0.f;
-  if (v >= 0) {
-    const T* hr = hc + i * ldc;
-    const T* wr = w + v * ldw;
-    for (int64_t c = lane * E; c < d; c += 64 * E) {
-      const uint4 a = *reinterpret_cast<const uint4*>(hr + c);
-      const T* x = reinterpret_cast<const T*>(&a);
-      if (c + E <= d) {
-        const uint4 b = ld16(wr + c);
-        const T* y = reinterpret_cast<const T*>(&b);
+// A row of n floats as split planes (padded to ld, pl elements apart) with the
+// exponent of its largest finite value, one wave; copy: also as it is.
+__device__ __forceinline__ void row_planes(const float* __restrict__ src, int64_t n, sp16* __restrict__ dst, int64_t pl,
+                                           int64_t ld, int* __restrict__ exponent, float* __restrict__ copy, int lane) {
+  float m = 0.f;
+  for (int64_t c = lane; c < n; c += 64) m = fabsf(src[c]) < INFINITY ? fmaxf(m, fabsf(src[c])) : m;
+  const int e = split_exp(wave_max(m));
+  if (lane == 0) *exponent = e;
+  for (int64_t c = lane * 8; c < ld; c += 512) {
+    float v[8];
 #pragma unroll
-        for (int q = 0; q < E; ++q) s = fmaf(to_f(x[q]), to_f(y[q]), s);
-      } else {
-        for (int q = 0; q < E; ++q)
-          if (c + q < d) s = fmaf(to_f(x[q]), to_f(wr[c + q]), s);
-      }
-    }
-    s = wave_sum(s) * scale;
+    for (int k = 0; k < 8; ++k) v[k] = c + k < n ? src[c + k] : 0.f;
+    if (copy) st8<float, float>(copy + c, v, 0, 8);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = ldexpf(v[k], e);
+    const Split8 s = split8(v);
+    *reinterpret_cast<uint4*>(dst + c) = s.h;
+    *reinterpret_cast<uint4*>(dst + pl + c) = s.l;
   }
-  if (lane == 0) out[(ch.base + i) * k + e] = s;
+}
+__global__ void __launch_bounds__(256) weight_planes_kernel(const float* __restrict__ w, int64_t ldw, int64_t vocab,
+                                                            int64_t d, sp16* __restrict__ out, int64_t ld,
+                                                            int* __restrict__ exponent) {
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r < vocab) row_planes(w + r * ldw, d, out + r * ld, vocab * ld, ld, exponent + r, nullptr, threadIdx.x & 63);
+}
+// gather_kernel for fp32: H as it is and as planes; also clears the maxima of
+// the chunk's columns.
+__global__ void __launch_bounds__(256) gather_planes_kernel(Chunk ch, const float* __restrict__ h, int64_t ldh,
+                                                            int64_t d, float* __restrict__ hc, int64_t ldc,
+                                                            sp16* __restrict__ planes, int64_t pl,
+                                                            int* __restrict__ exponent, float* __restrict__ dh,
+                                                            unsigned* __restrict__ maxima, int64_t nmax) {
+  const int lane = threadIdx.x & 63;
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < nmax; c += (int64_t)gridDim.x * 256) maxima[c] = 0;
+  if (i < ch.live())
+    row_planes(h + ch.list[ch.base + i] * ldh, d, planes + i * ldc, pl, ldc, exponent + i, hc + i * ldc, lane);
+  else if (i < ch.padded())
+    copy_row(h, 0, hc + i * ldc, ldc, lane);
+  if (dh && i >= ch.live() && i < ch.cap) zero_row(dh + ch.list[ch.base + i] * d, d, lane);
 }
 
 // 2^x of one v_exp_f32 (1 ulp; results below 2^-126 are 0).
@@ -299,14 +391,15 @@ __device__ __forceinline__ float sum16(float v) {
   return v + dpp<0x140>(v);
 }
 
-// What a row's slopes need besides its logits: S = pa·2^(t − lse2) + pu.
+// What a row's slopes need besides its logits t (in log2): S = pa·2^(t − m) + pu.
 struct RowSlope {
-  float lse2, pa, pu;
+  float m, pa, pu;
 };
 
 // Epilogue of the logits' product, from the accumulators (kDirect): 16 lanes
 // have a row's 64 columns, four each. Through LDS staging in runs of eight the
 // same work took 14 us of a 256² tile's 69 at d = 2048, most of it VALU.
+// fp32 inputs come as split operands, with a power of two per row of each.
 template <typename T, bool KEEP, bool SLOPE>
 struct EpiLogits {
   typedef float S;
@@ -320,6 +413,10 @@ struct EpiLogits {
   void* kept;      // KEEP: the kept logits (uint16_t or float); SLOPE: S
   int64_t ld;
   const RowSlope* row;
+  const int *eh, *ew;  // fp32: the exponents of the rows of H and W
+  Targets tg;
+  int k;
+  float* targets;  // [cap][k], null: the targets' logits t, by rank
   __device__ __forceinline__ bool adjust(GemmArgs& g, int, int row0, int) const {
     g.M = SLOPE ? ch.padded() : ch.live();
     return row0 < g.M;
@@ -333,12 +430,35 @@ struct EpiLogits {
     const int l = lane & 15, sub = (lane >> 4) * 4, c0 = wc0 + 4 * l;
     const bool whole = wc0 + kCols <= vocab;  // false in the last block of a row at most
     RowSlope* const rs = reinterpret_cast<RowSlope*>(lds);
-    if (SLOPE) {
-      for (int r = lane; r < FM * 16; r += 64)
-        if (wr0 + r < g.M) rs[r] = row[wr0 + r];
-      __builtin_amdgcn_s_waitcnt(PTO_LGKM0);
-      __builtin_amdgcn_wave_barrier();
+    constexpr int R = FM * 16;
+    unsigned long long* const bits = reinterpret_cast<unsigned long long*>(lds);  // one: the row's token
+    uint16_t* const before = reinterpret_cast<uint16_t*>(bits + R);
+    int* const er = reinterpret_cast<int*>(before + R);
+    int ec[4] = {0, 0, 0, 0};
+    if (targets) {
+      const int64_t b = wc0 / kCols;
+      for (int r = lane; r < R; r += 64) {
+        const int i = wr0 + r;
+        const bool live = i < g.M;
+        if (tg.one) {
+          bits[r] = live ? (unsigned)tg.one[ch.base + i] : ~0u;
+        } else {
+          bits[r] = live ? tg.bits[b * ch.cap + i] : 0;
+          before[r] = live ? tg.before[b * ch.cap + i] : 0;
+        }
+      }
     }
+    if (sizeof(T) == 4) {
+      for (int r = lane; r < R; r += 64) er[r] = eh[min(wr0 + r, g.M - 1)];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) ec[k] = ew[min(c0 + k, vocab - 1)];
+    }
+    if (SLOPE) {
+      for (int r = lane; r < R; r += 64)
+        if (wr0 + r < g.M) rs[r] = row[wr0 + r];
+    }
+    __builtin_amdgcn_s_waitcnt(PTO_LGKM0);
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
 #pragma unroll
@@ -348,11 +468,16 @@ struct EpiLogits {
         float v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = acc[fm][k][r];
+        if (sizeof(T) == 4) {
+          const int e = er[fm * 16 + sub + r];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = ldexpf(v[k], -e - ec[k]);
+        }
         if (SLOPE) {
           const RowSlope p = rs[fm * 16 + sub + r];
           float t[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) t[k] = fmaf(p.pa, pow2(fmaf(v[k], scale, -p.lse2)), p.pu);
+          for (int k = 0; k < 4; ++k) t[k] = fmaf(p.pa, pow2(fmaf(v[k], scale, -p.m)), p.pu);
           if (!whole) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) t[k] = c0 + k < vocab ? t[k] : 0.f;
@@ -364,6 +489,7 @@ struct EpiLogits {
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] = c0 + k < vocab ? v[k] : -INFINITY;
         }
+        if (targets) catch_targets(v, bits[fm * 16 + sub + r], before[fm * 16 + sub + r], i, wc0, l);
         const float m = max16(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
         const float ref = m == -INFINITY ? 0.f : m * scale;  // a block of nothing but -inf sums to 0
         float x[4], s = 0.f;
@@ -397,6 +523,25 @@ struct EpiLogits {
       }
     }
   }
+  // The targets among a lane's four columns of a row.
+  __device__ __forceinline__ void catch_targets(const float (&v)[4], unsigned long long word, int first, int64_t i,
+                                                int wc0, int l) const {
+    if (tg.one) {
+      const unsigned at = (unsigned)word - wc0;  // -2 and left-out rows: past every block
+      if (at < kCols && (int)(at >> 2) == l) {
+        const int c = at & 3;
+        targets[i] = (c == 0 ? v[0] : c == 1 ? v[1] : c == 2 ? v[2] : v[3]) * scale;
+      }
+      return;
+    }
+    const unsigned mine = (unsigned)(word >> (4 * l)) & 15u;
+    if (mine) {
+      int64_t to = i * k + first + __popcll(word & ((1ull << (4 * l)) - 1));
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (mine >> c & 1) targets[to++] = v[c] * scale;
+    }
+  }
   // (x/128 + 1)·65535, rounded, between 0 and 65535
   __device__ __forceinline__ static unsigned encode(float a, float b) {
     return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(fmaf(a, 1.f / kOctaves, 1.f),
@@ -420,54 +565,74 @@ struct LossSpec {
   float lambda;   // T² (1 for cross entropy)
   float smooth;   // ε/V
   float zeta;
-  float inv_temp;
   int k;
-  int reduction;  // 0: gradients (if any) under grad_rows, 1: mean, 2: sum
 };
 
-// a and f of a row (see the top), as the slope of exp2(t - lse2) and the constant.
-__device__ __forceinline__ RowSlope row_slope(const LossSpec& sp, float lse2, float g) {
+// Where the logits overflow, or a target is outside the vocabulary or not a
+// number, nothing of the row is left standing as a number.
+__device__ __forceinline__ bool sound(float x) { return fabsf(x) < INFINITY; }
+
+// A row of S, times a.
+__device__ __forceinline__ RowSlope row_slope(const LossSpec& sp, float2 norm, float qz, float a) {
+  const float lse2 = norm.x + log2f(norm.y);
   RowSlope r;
-  r.lse2 = lse2;
-  const float a = g * sp.lambda * sp.inv_temp;
-  r.pa = a * (1.f + 2.f * sp.zeta * (float)(kLn2 * lse2));
-  // where the logits overflow nothing of the row is left standing as a number
-  if (!(fabsf(lse2) < INFINITY)) r.pa = NAN;
+  r.m = norm.x;
+  r.pa = sound(lse2) && sound(qz) ? a * (1.f + 2.f * sp.zeta * (float)(kLn2 * lse2)) / norm.y : NAN;
   r.pu = -a * sp.smooth;
   return r;
 }
-
+// S at a sparse target with logit z, S being scaled by a.
+__device__ __forceinline__ float at_target(const RowSlope& rs, float a, float put, float z) {
+  return fmaf(rs.pa, pow2(z - rs.m), fmaf(-a, put, rs.pu));
+}
 // S at a row's sparse targets, after the dense part was written.
-template <typename T>
-__device__ __forceinline__ void put_targets(T* srow, const RowSlope& rs, const LossSpec& sp, float g, const int* id,
-                                            const float* put, const float* z, int first, int step) {
-  const float a = g * sp.lambda * sp.inv_temp;
-  for (int e = first; e < sp.k; e += step)
-    if (id[e] >= 0 && put[e] >= 0.f) srow[id[e]] = T(fmaf(rs.pa, pow2(z[e] - rs.lse2), fmaf(-a, put[e], rs.pu)));
+__device__ __forceinline__ void put_targets(bf16* srow, const RowSlope& rs, float a, const RowTargets& t,
+                                            const float* z, int first, int step) {
+  for (int e = first; e < t.k; e += step)
+    if (t.id(e) >= 0 && t.put(e) >= 0.f) srow[t.id(e)] = bf16(at_target(rs, a, t.put(e), z[e]));
 }
 
-// One workgroup per listed row: lse, the loss and (S not null) S in place of
-// the kept logits. losses is per row of the call, lse2_out per listed row.
+// fp32: S/a of a row, its a, and the largest |S/a| of every column, as bits.
+struct RowsOut {
+  RowSlope* slope;
+  float* a;
+  unsigned* maxima;
+  __device__ __forceinline__ void put(int i, const LossSpec& sp, float2 norm, float qz, float av, const RowTargets& t,
+                                      const float* z, int first, int step) const {
+    const RowSlope rs = row_slope(sp, norm, qz, 1.f);
+    if (first == 0) {
+      slope[i] = rs;
+      a[i] = av;
+    }
+    for (int e = first; e < t.k; e += step)
+      if (t.id(e) >= 0 && t.put(e) >= 0.f) {
+        const float v = fabsf(at_target(rs, 1.f, t.put(e), z[e]));
+        if (v < INFINITY) atomicMax(&maxima[t.id(e)], __float_as_uint(v));
+      }
+  }
+};
+
+// One workgroup per listed row: the normaliser, the loss and, for gradients
+// (SLOPES), S/alpha in place of the kept logits (bf16) or what the passes over
+// them need (fp32). losses is per row of the call; norm (m, s) and z (the
+// targets' logits in the caller's order) per listed row.
 template <typename T, bool SLOPES>
 __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __restrict__ stats,
                                                      const float* __restrict__ sums, int64_t blocks, LossSpec sp,
-                                                     Targets tg, const float* __restrict__ z, int vocab,
-                                                     void* __restrict__ kept, int64_t ld, float* __restrict__ losses,
-                                                     float* __restrict__ lse2_out) {
+                                                     Targets tg, const float* __restrict__ caught, int vocab,
+                                                     bf16* __restrict__ kept, int64_t ld, RowsOut out,
+                                                     const float* __restrict__ alpha, float* __restrict__ losses,
+                                                     float2* __restrict__ norms, float* __restrict__ z) {
   const int i = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int live = ch.live();
-  constexpr int E = 16 / (int)sizeof(T);
-  if (i >= live) {
-    if (SLOPES && i < ch.padded())
-      for (int64_t c = tid * E; c < ld; c += 256 * E)
-        *reinterpret_cast<uint4*>(static_cast<T*>(kept) + i * ld + c) = make_uint4(0, 0, 0, 0);
+  if (i >= ch.live()) {
+    if (SLOPES && sizeof(T) == 2 && i < ch.padded())
+      for (int64_t c = tid * 8; c < ld; c += 2048) *reinterpret_cast<uint4*>(kept + i * ld + c) = make_uint4(0, 0, 0, 0);
     return;
   }
   const int row = ch.list[ch.base + i];
   const float2* st = stats + i * blocks;
-  const int* id = tg.id + (int64_t)row * sp.k;
-  const float* q = tg.q + (int64_t)row * sp.k;
-  const float* zr = z + (int64_t)(ch.base + i) * sp.k;
+  const RowTargets rt{tg, ch.base + i, row, sp.k};
+  float* zr = z + (int64_t)(ch.base + i) * sp.k;
   __shared__ float red[4][4];
   float m = -INFINITY;
   for (int64_t c = tid; c < blocks; c += 256)
@@ -477,13 +642,21 @@ __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __r
   __syncthreads();
   m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   if (m == -INFINITY) m = 0.f;
+  // targets around m: what is summed is small where the row is right
   float s = 0.f, sz = 0.f, qz = 0.f;
   for (int64_t c = tid; c < blocks; c += 256) {
-    s += st[c].y == 0.f ? 0.f : st[c].y * pow2(st[c].x - m);
-    if (sums) sz += sums[i * blocks + c];
+    s += st[c].y == 0.f ? 0.f : st[c].y * exp2f(st[c].x - m);
+    if (sums) sz += sums[i * blocks + c] - m * (float)max((int64_t)0, min((int64_t)kCols, vocab - c * kCols));
   }
-  for (int e = tid; e < sp.k; e += 256)
-    if (id[e] != -1) qz += q[e] * zr[e];
+  for (int e = tid; e < sp.k; e += 256) {
+    const int id = rt.id(e);
+    float ze = 0.f;
+    if (id != -1) {
+      ze = id < 0 ? NAN : caught[tg.one ? i : (int64_t)i * sp.k + tg.rank[(int64_t)i * sp.k + e]];
+      qz += rt.q(e) * (ze - m);
+    }
+    zr[e] = ze;
+  }
   s = wave_sum(s);
   sz = wave_sum(sz);
   qz = wave_sum(qz);
@@ -496,74 +669,74 @@ __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __r
   s = red[1][0] + red[1][1] + red[1][2] + red[1][3];
   sz = red[2][0] + red[2][1] + red[2][2] + red[2][3];
   qz = red[3][0] + red[3][1] + red[3][2] + red[3][3];
-  const float lse2 = m + log2f(s);
+  const float2 norm = make_float2(m, s);
   if (tid == 0) {
-    const double lse = kLn2 * ((double)m + (double)log2f(s));
-    const double nat = lse - kLn2 * ((double)qz + (double)sp.smooth * sz) + tg.entropy[row];
+    const double logs = log2((double)s);
+    const double nat = kLn2 * (logs - ((double)qz + (double)sp.smooth * sz)) + rt.entropy();
+    const double lse = kLn2 * ((double)m + logs);
     losses[row] = (float)(sp.lambda * nat + (double)sp.zeta * lse * lse);
-    if (lse2_out) lse2_out[ch.base + i] = lse2;
+    norms[ch.base + i] = norm;
   }
   if constexpr (SLOPES) {
-    const float g = sp.reduction == 1 ? 1.f / (float)ch.count[0] : 1.f;
-    RowSlope rs = row_slope(sp, lse2, g);
-    if (!(fabsf(qz) < INFINITY)) rs.pa = NAN;  // a target outside the vocabulary, or one that is not a number
-    for (int64_t c = tid * E; c < ld; c += 256 * E) {
-      float o[E];
-      if constexpr (sizeof(T) == 2) {
-        const uint4 u = *reinterpret_cast<const uint4*>(static_cast<uint16_t*>(kept) + i * ld + c);
-        const unsigned uw[4] = {u.x, u.y, u.z, u.w};
-        const float off = st[c / kCols].x - rs.lse2 - kOctaves;
+    if constexpr (sizeof(T) == 4) {
+      out.put(i, sp, norm, qz, alpha[0], rt, zr, tid, 256);
+      return;
+    }
+    const RowSlope rs = row_slope(sp, norm, qz, 1.f);
+    for (int64_t c = tid * 8; c < ld; c += 2048) {
+      const uint4 u = *reinterpret_cast<const uint4*>(kept + i * ld + c);
+      const unsigned uw[4] = {u.x, u.y, u.z, u.w};
+      const float off = (st[c / kCols].x - m) - kOctaves;
+      float o[8];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const unsigned x = e & 1 ? uw[e / 2] >> 16 : uw[e / 2] & 0xffffu;
-          const float p = x ? pow2(fmaf((float)x, kOctaves / 65535.f, off)) : 0.f;
-          o[e] = c + e < vocab ? fmaf(rs.pa, p, rs.pu) : 0.f;
-        }
-        uint4 r;
-        T* re = reinterpret_cast<T*>(&r);
-#pragma unroll
-        for (int e = 0; e < E; ++e) re[e] = T(o[e]);
-        *reinterpret_cast<uint4*>(static_cast<T*>(kept) + i * ld + c) = r;
-      } else {
-        float* p = static_cast<float*>(kept) + i * ld + c;
-        const float4 x = *reinterpret_cast<const float4*>(p);
-        const float xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = c + e < vocab ? fmaf(rs.pa, pow2(xs[e] - rs.lse2), rs.pu) : 0.f;
-        *reinterpret_cast<float4*>(p) = make_float4(o[0], o[1], o[2], o[3]);
+      for (int e = 0; e < 8; ++e) {
+        const unsigned x = e & 1 ? uw[e / 2] >> 16 : uw[e / 2] & 0xffffu;
+        const float p = x ? pow2(fmaf((float)x, kOctaves / 65535.f, off)) : 0.f;
+        o[e] = c + e < vocab ? fmaf(rs.pa, p, rs.pu) : 0.f;
       }
+      st8<bf16, float>(kept + i * ld + c, o, 0, 8);
     }
     __syncthreads();  // the dense part is written before the targets' entries replace theirs
-    put_targets(static_cast<T*>(kept) + i * ld, rs, sp, g, id, tg.put + (int64_t)row * sp.k, zr, tid, 256);
+    put_targets(kept + i * ld, rs, 1.f, rt, zr, tid, 256);
   }
 }
 
-// Gradients of losses per row: what the logits' epilogue needs of each row
-// (zero for the pad rows).
-__global__ void __launch_bounds__(256) row_slopes_kernel(Chunk ch, LossSpec sp, Targets tg, const float* __restrict__ z,
-                                                         const float* __restrict__ lse2,
-                                                         const float* __restrict__ grad_rows, RowSlope* out) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= ch.padded()) return;
-  RowSlope rs{0.f, 0.f, 0.f};
-  if (i < ch.live()) {
-    const int64_t at = ch.base + i, row = ch.list[at];
-    rs = row_slope(sp, lse2[at], grad_rows[row]);
-    for (int e = 0; e < sp.k; ++e)
-      if (tg.id[row * sp.k + e] != -1 && !(fabsf(tg.q[row * sp.k + e] * z[at * sp.k + e]) < INFINITY)) rs.pa = NAN;
-  }
-  out[i] = rs;
-}
+// Gradients of losses per row, normaliser and targets' logits kept: what the
+// logits' epilogue (bf16: S/alpha) or the passes over them (fp32) need of each
+// row; pad rows 0. One wave per row.
 template <typename T>
-__global__ void __launch_bounds__(64) put_targets_kernel(Chunk ch, LossSpec sp, Targets tg, const float* __restrict__ z,
-                                                         const RowSlope* __restrict__ rows,
-                                                         const float* __restrict__ grad_rows, T* __restrict__ s,
-                                                         int64_t ld) {
+__global__ void __launch_bounds__(256) row_slopes_kernel(Chunk ch, LossSpec sp, Targets tg, const float* __restrict__ z,
+                                                         const float2* __restrict__ norms,
+                                                         const float* __restrict__ grad_rows, float scale,
+                                                         const float* __restrict__ alpha, RowsOut out) {
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (i >= ch.padded()) return;
+  if (i >= ch.live()) {
+    if (lane == 0) out.slope[i] = RowSlope{0.f, 0.f, 0.f};
+    return;
+  }
+  const int64_t at = ch.base + i, row = ch.list[at];
+  const RowTargets rt{tg, at, row, sp.k};
+  const float* zr = z + at * sp.k;
+  const float2 norm = norms[at];
+  float qz = 0.f;
+  for (int e = lane; e < sp.k; e += 64)
+    if (rt.id(e) != -1) qz += rt.q(e) * (zr[e] - norm.x);
+  qz = wave_sum(qz);
+  const float a = grad_rows[row] * scale;
+  if constexpr (sizeof(T) == 4) {
+    out.put(i, sp, norm, qz, a, rt, zr, lane, 64);
+  } else if (lane == 0) {
+    out.slope[i] = row_slope(sp, norm, qz, a / alpha[0]);
+    out.a[i] = a / alpha[0];
+  }
+}
+__global__ void __launch_bounds__(64) put_targets_kernel(Chunk ch, int k, Targets tg, const float* __restrict__ z,
+                                                         RowsOut rows, bf16* __restrict__ s, int64_t ld) {
   const int i = blockIdx.x;
   if (i >= ch.live()) return;
-  const int64_t at = ch.base + i, row = ch.list[at];
-  put_targets(s + i * ld, rows[i], sp, grad_rows[row], tg.id + row * sp.k, tg.put + row * sp.k, z + at * sp.k,
-              threadIdx.x, 64);
+  const int64_t at = ch.base + i;
+  put_targets(s + i * ld, rows.slope[i], rows.a[i], RowTargets{tg, at, ch.list[at], k}, z + at * k, threadIdx.x, 64);
 }
 
 // The loss of the call: a sum in a fixed order, over the count for the mean
@@ -573,6 +746,7 @@ __global__ void __launch_bounds__(1024) reduce_loss_kernel(const float* __restri
                                                            float* __restrict__ out) {
   __shared__ double red[1024];
   double s = 0;
+#pragma unroll 8
   for (int64_t r = threadIdx.x; r < rows; r += 1024) s += losses[r];
   red[threadIdx.x] = s;
   __syncthreads();
@@ -580,87 +754,170 @@ __global__ void __launch_bounds__(1024) reduce_loss_kernel(const float* __restri
     if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
     __syncthreads();
   }
-  if (threadIdx.x == 0) out[0] = (float)(red[0] / (mean ? max(1, count[0]) : 1));
+  if (threadIdx.x == 0) out[0] = (float)(red[0] / (mean && rows ? max(1, count[0]) : 1));
+}
+
+// fp32: S/a and a·H as split planes for the gradients' products. dW sums over
+// the rows, so a column of each has an exponent of its own, from its largest
+// value: tokens that are unlikely in every row keep their bits. dH sums over
+// the vocabulary, with the columns' exponents taken out of W's rows
+// (launch_split_pack_max); a, which may differ by rows, multiplies its result.
+
+// Largest values of 1024 columns over 64 rows: of S/a (EXP, x = the logits) or
+// of a·x.
+template <bool EXP>
+__global__ void __launch_bounds__(256) column_max_kernel(Chunk ch, const float* __restrict__ x, int64_t ld, int cols,
+                                                         const RowSlope* __restrict__ slope,
+                                                         const float* __restrict__ a, unsigned* __restrict__ maxima) {
+  const int c = (blockIdx.x * 256 + threadIdx.x) * 4, r0 = blockIdx.y * 64, r1 = min(r0 + 64, ch.live());
+  if (c >= cols) return;
+  float m[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = r0; i < r1; ++i) {
+    const float4 t = *reinterpret_cast<const float4*>(x + i * ld + c);
+    const float v[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float w = fabsf(EXP ? fmaf(slope[i].pa, pow2(v[k] - slope[i].m), slope[i].pu) : a[i] * v[k]);
+      m[k] = w < INFINITY ? fmaxf(m[k], w) : m[k];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (c + k < cols && r0 < r1) atomicMax(&maxima[c + k], __float_as_uint(m[k]));
+}
+__global__ void __launch_bounds__(256) exponents_kernel(const unsigned* __restrict__ maxima, int64_t n,
+                                                        int* __restrict__ e) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c < n) e[c] = split_exp(__uint_as_float(maxima[c]));
+}
+// The planes, one workgroup per row; pad rows and columns 0.
+template <bool EXP>
+__global__ void __launch_bounds__(256) column_planes_kernel(Chunk ch, const float* __restrict__ x, int64_t ld, int cols,
+                                                            const RowSlope* __restrict__ slope,
+                                                            const float* __restrict__ a, const int* __restrict__ ec,
+                                                            sp16* __restrict__ out, int64_t pl, int k, Targets tg,
+                                                            const float* __restrict__ z) {
+  const int i = blockIdx.x, tid = threadIdx.x;
+  if (i >= ch.padded()) return;
+  const bool live = i < ch.live();
+  sp16* o = out + i * ld;
+  const RowSlope rs = EXP && live ? slope[i] : RowSlope{0.f, 0.f, 0.f};
+  const float ai = !EXP && live ? a[i] : 0.f;
+  for (int64_t c = tid * 8; c < ld; c += 2048) {
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const float4 t = live ? *reinterpret_cast<const float4*>(x + i * ld + c + 4 * q) : make_float4(0, 0, 0, 0);
+      v[4 * q] = t.x;
+      v[4 * q + 1] = t.y;
+      v[4 * q + 2] = t.z;
+      v[4 * q + 3] = t.w;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float w = EXP ? fmaf(rs.pa, pow2(v[k] - rs.m), rs.pu) : ai * v[k];
+      v[k] = live && c + k < cols ? ldexpf(w, ec[c + k]) : 0.f;
+    }
+    const Split8 s = split8(v);
+    *reinterpret_cast<uint4*>(o + c) = s.h;
+    *reinterpret_cast<uint4*>(o + pl + c) = s.l;
+  }
+  if constexpr (EXP) {
+    if (!live) return;
+    __syncthreads();
+    const int64_t at = ch.base + i;
+    const RowTargets rt{tg, at, ch.list[at], k};
+    for (int e = tid; e < k; e += 256) {
+      const int id = rt.id(e);
+      if (id < 0 || !(rt.put(e) >= 0.f)) continue;
+      const float w = ldexpf(at_target(rs, 1.f, rt.put(e), z[at * k + e]), ec[id]);
+      const _Float16 h = static_cast<_Float16>(w);
+      o[id].v = h;
+      o[pl + id].v = static_cast<_Float16>(w - static_cast<float>(h));
+    }
+  }
 }
 
 // ------------------------------------------------------------ gradients
 
-// dH: rows of the chunk to their places.
-template <typename T>
-struct EpiRows {
+// What the three epilogues below share: no transposed pass, nothing read early.
+struct EpiPlain {
   typedef float S;
-  Chunk ch;
-  T* dst;
-  int64_t ld;
   typedef NoPre Pre;
   typedef NoPre PreT;
   static constexpr bool kVoIsV = true;
   __device__ __forceinline__ bool has_t() const { return false; }
-  __device__ __forceinline__ bool adjust(GemmArgs& g, int, int row0, int) const {
-    g.M = ch.live();
-    return row0 < g.M;
-  }
   __device__ __forceinline__ void load(int, int, int, int, int, Pre&) const {}
   __device__ __forceinline__ void load_t(int, int, int, int, PreT&) const {}
   __device__ __forceinline__ void put_t(int, int, int, const S*, int, const PreT&) const {}
   __device__ __forceinline__ void finish(int) const {}
+};
+
+// dH: rows of the chunk to their places, times what S is without: alpha, or
+// each row's a (fp32).
+template <typename T>
+struct EpiRows : EpiPlain {
+  Chunk ch;
+  T* dst;
+  int64_t ld;
+  const float* a;
+  __device__ __forceinline__ bool adjust(GemmArgs& g, int, int row0, int) const {
+    g.M = ch.live();
+    return row0 < g.M;
+  }
   __device__ __forceinline__ void put(int, int i, int j0, const S* v, int kbeg, int n, const Pre&, S*) const {
-    st8<T, S>(dst + ch.list[ch.base + i] * ld + j0, v, kbeg, n);
+    const float f = a[sizeof(T) == 4 ? i : 0];
+    S w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = v[k] * f;
+    st8<T, S>(dst + ch.list[ch.base + i] * ld + j0, w, kbeg, n);
   }
 };
 
 // dH of few rows: the vocabulary split over the batch index, partial sums to
 // the workspace.
-struct EpiPart {
-  typedef float S;
+struct EpiPart : EpiPlain {
   Chunk ch;
   float* dst;
   int64_t ld, sd;
   int len, total;  // K of a slice, of all
-  typedef NoPre Pre;
-  typedef NoPre PreT;
-  static constexpr bool kVoIsV = true;
-  __device__ __forceinline__ bool has_t() const { return false; }
   __device__ __forceinline__ bool adjust(GemmArgs& g, int b, int row0, int) const {
     g.M = ch.live();
     g.K = max(0, min(len, total - b * len));
     return row0 < g.M;
   }
-  __device__ __forceinline__ void load(int, int, int, int, int, Pre&) const {}
-  __device__ __forceinline__ void load_t(int, int, int, int, PreT&) const {}
-  __device__ __forceinline__ void put_t(int, int, int, const S*, int, const PreT&) const {}
-  __device__ __forceinline__ void finish(int) const {}
   __device__ __forceinline__ void put(int b, int i, int j0, const S* v, int kbeg, int n, const Pre&, S*) const {
     st8<float, S>(dst + b * sd + i * ld + j0, v, kbeg, n);
   }
 };
 template <typename T>
 __global__ void __launch_bounds__(256) join_parts_kernel(Chunk ch, const float* __restrict__ part, int64_t ld,
-                                                         int64_t sd, int parts, int64_t d, T* __restrict__ dst) {
+                                                         int64_t sd, int parts, int64_t d, const float* __restrict__ a,
+                                                         T* __restrict__ dst) {
   const int i = blockIdx.x;
   if (i >= ch.live()) return;
+  const float f = a[sizeof(T) == 4 ? i : 0];
   T* row = dst + ch.list[ch.base + i] * d;
   for (int64_t c = threadIdx.x; c < d; c += 256) {
     float s = 0.f;
+#pragma unroll 8
     for (int p = 0; p < parts; ++p) s += part[p * sd + i * ld + c];
-    row[c] = convert<T>(s);
+    row[c] = convert<T>(s * f);
   }
 }
 
-// dW over the chunks of rows: acc = v (first), acc + v, and out = acc + v
-// rounded (last); acc is out where the chunk is the only one or out is fp32.
+// dW over the chunks of rows: acc = v (first), acc + v, and out = acc + v,
+// times alpha (bf16) and rounded (last); acc is out where the chunk is the only one or out is fp32.
 template <typename T>
-struct EpiWeight {
-  typedef float S;
+struct EpiWeight : EpiPlain {
   Chunk ch;
   float* acc;
   T* out;
   int64_t ld;
   int first, last;
+  const float* alpha;
   typedef Raw8<float> Pre;
-  typedef NoPre PreT;
-  static constexpr bool kVoIsV = true;
-  __device__ __forceinline__ bool has_t() const { return false; }
   __device__ __forceinline__ bool adjust(GemmArgs& g, int, int, int) const {
     g.K = ch.padded();
     return g.K > 0 || first || last;
@@ -668,9 +925,6 @@ struct EpiWeight {
   __device__ __forceinline__ void load(int, int i, int j0, int kbeg, int n, Pre& p) const {
     if (!first) ld8_pre<float>(acc + i * ld + j0, p, kbeg, n);
   }
-  __device__ __forceinline__ void load_t(int, int, int, int, PreT&) const {}
-  __device__ __forceinline__ void put_t(int, int, int, const S*, int, const PreT&) const {}
-  __device__ __forceinline__ void finish(int) const {}
   __device__ __forceinline__ void put(int, int i, int j0, const S* v, int kbeg, int n, const Pre& p, S*) const {
     float r[8];
     if (first) {
@@ -681,10 +935,45 @@ struct EpiWeight {
 #pragma unroll
       for (int k = 0; k < 8; ++k) r[k] += v[k];
     }
+    if (last && sizeof(T) == 2) {
+      const float f = alpha[0];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) r[k] *= f;
+    }
     if (last)
       st8<T, float>(out + i * ld + j0, r, kbeg, n);
     else
       st8<float, float>(acc + i * ld + j0, r, kbeg, n);
+  }
+};
+
+// One of them over split operands: the powers of two of the rows (er, or none)
+// and columns taken out first.
+template <class In>
+struct EpiPowers {
+  typedef float S;
+  typedef typename In::Pre Pre;
+  typedef NoPre PreT;
+  static constexpr bool kVoIsV = true;
+  In in;
+  const int *er, *ec;
+  int off;
+  __device__ __forceinline__ bool has_t() const { return false; }
+  __device__ __forceinline__ bool adjust(GemmArgs& g, int b, int row0, int col0) const {
+    return in.adjust(g, b, row0, col0);
+  }
+  __device__ __forceinline__ void load(int b, int i, int j0, int kbeg, int n, Pre& p, bool) const {
+    in.load(b, i, j0, kbeg, n, p);
+  }
+  __device__ __forceinline__ void load_t(int, int, int, int, PreT&, bool) const {}
+  __device__ __forceinline__ void put_t(int, int, int, const S*, int, const PreT&, bool) const {}
+  __device__ __forceinline__ void finish(int) const {}
+  __device__ __forceinline__ void put(int b, int i, int j0, const S* v, int kbeg, int n, const Pre& p, S*, bool) const {
+    S w[8], drop[8];
+    const int e = off - (er ? er[i] : 0);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = k < n ? ldexpf(v[k], e - ec[j0 + k]) : 0.f;
+    in.put(b, i, j0, w, kbeg, n, p, drop);
   }
 };
 
@@ -716,6 +1005,7 @@ struct Call {
   int64_t ldh;
   const void* w;
   int64_t ldw;
+  bool kd;
   const int64_t* y;       // cross entropy
   int64_t ignore;
   const float* teacher;   // distillation
@@ -724,29 +1014,35 @@ struct Call {
   double temp, smooth, zeta;
   int reduction;
   const float* grad_rows;
-  float *loss, *lse, *z;
+  float *loss, *norm, *z;
   void *dh, *dw;
   int64_t chunk_bytes;
   const char* name;
 };
 
+// Operand type of a dtype's products.
+template <typename T>
+using Operand = std::conditional_t<sizeof(T) == 4, sp16, bf16>;
+
 // Parts of the vocabulary that dH of a chunk is split into: as many as leave
 // no CU idle through a long loop over K, each at least kPadK deep; the partial
-// sums (8 bytes of traffic an element) count against it.
+// sums (8 bytes of traffic an element) count against it. *tile: the faster
+// tile (pick_tile's 0 or 1).
 template <typename T>
 int grad_parts(int64_t rows, int64_t d, int64_t vp, int* tile) {
-  typedef typename TileSet<T>::big Big;
-  typedef typename TileSet<T>::small Small;
+  typedef TileSet<Operand<T>> Set;
+  typedef typename Set::big Big;
+  typedef typename Set::small Small;
   const int64_t cus = device_cus(), units = vp / kPadK;
-  // microseconds of one unit of K on one CU, per element of a tile
-  const double us = sizeof(T) == 2 ? 3.6 / 65536 : 5.0 / 16384;
+  // microseconds of one unit of K on one CU, per element of a 256² tile
+  const double us = (sizeof(T) == 2 ? 3.6 : 8.25) / 65536;
   double best = 0;
   int parts = 1;
   for (int big = 0; big < 2; ++big) {
     const int64_t bm = big ? Big::BM : Small::BM, bn = big ? Big::BN : Small::BN;
     const int64_t tiles = ((rows + bm - 1) / bm) * ((d + bn - 1) / bn);
     for (int p = 1; p <= 64 && p <= units; p *= 2) {
-      const double unit = bm * bn * us * (big ? 1.0 : TileSet<T>::kBigRate);
+      const double unit = bm * bn * us * (big ? 1.0 : Set::kBigRate);
       double t = double((tiles * p + cus - 1) / cus) * ((units + p - 1) / p) * unit;
       if (p > 1) t += 5 + p * (double)rows * d * 8 / 4e6;
       if ((!big && p == 1) || t < best) {
@@ -761,49 +1057,88 @@ int grad_parts(int64_t rows, int64_t d, int64_t vp, int* tile) {
 
 template <typename T>
 struct Ws {
+  static constexpr bool f32 = sizeof(T) == 4;
   int64_t dp, vp, blocks, cap, capp;
   bool pad_w;
-  int parts, part_tile = 0;
-  Targets t;
+  int parts, part_tile = 0, part_len;
+  Targets t{};
   int *list, *count;
-  T *hc, *wp;
-  float2* stats;
-  float *sums, *losses, *lse, *z;
-  RowSlope* slopes;
-  void* kept;
-  T *keptT, *hcT, *wT;
+  T* hc;
+  bf16* wp;  // bf16: W padded
+  float2 *stats, *norm;
+  float *sums, *losses, *z, *caught, *alpha;
+  RowsOut rows;
+  T* kept;  // the kept logits, bf16: then S
+  // fp32: planes of H and W (by rows) for the logits, of S/a, W (transposed,
+  // S's exponents taken out) and a·H (by columns) for the gradients
+  sp16 *hp, *wpl, *sp, *wt, *ah;
+  int *eh, *ew, *es, *ewt, *eah;  // es and eah: exponents of the columns' maxima
+  unsigned* wpart;
   float *part, *acc;
   int64_t chunks(const Call& c) const { return c.rows ? (c.rows + cap - 1) / cap : 0; }
   Ws(Carver& cv, const Call& c) {
-    const bool f32 = sizeof(T) == 4, grads = c.dh || c.dw;
+    const bool grads = c.dh || c.dw;
     dp = round_up(c.d, kPadK);
     vp = round_up(c.vocab, kPadK);
     blocks = vp / kCols;
-    const int64_t per = grads ? vp * (int64_t)sizeof(T) * (f32 && c.dw ? 2 : 1) : blocks * 8;
+    const int64_t per = grads ? vp * (f32 ? 8 : 2) : blocks * 8;
     cap = (c.chunk_bytes > 0 ? c.chunk_bytes : kChunkBytes) / per;
     cap = std::min(std::max<int64_t>(cap / 256 * 256, 256), std::max<int64_t>(c.rows, 1));
     capp = round_up(cap, kPadK);
-    pad_w = c.d % kPadK || c.ldw % (16 / sizeof(T)) || (!f32 && c.dh && c.vocab % kPadK);
-    t.id = cv.take<int>(c.rows * c.k);
-    t.q = cv.take<float>(c.rows * c.k);
-    t.put = cv.take<float>(c.rows * c.k);
-    t.entropy = cv.take<float>(c.rows);
-    t.kept = cv.take<int>(c.rows);
+    pad_w = !f32 && (c.d % kPadK || c.ldw % 8 || (c.dh && c.vocab % kPadK));
+    const bool join = !c.grad_rows;
+    if (c.kd) {
+      t.id = cv.take<int>(c.rows * c.k);
+      t.q = cv.take<float>(c.rows * c.k);
+      t.put = cv.take<float>(c.rows * c.k);
+      t.entropy = cv.take<float>(c.rows);
+      t.kept = cv.take<int>(c.rows);
+      t.rank = cv.take<uint16_t>(cap * c.k);
+    } else {
+      t.one = cv.take<int>(c.rows);
+      t.share = (float)(1.0 - c.smooth);
+    }
+    if (c.kd && join) {
+      t.bits = cv.take<unsigned long long>(blocks * cap);
+      t.before = cv.take<uint16_t>(blocks * cap);
+    }
     list = cv.take<int>(c.rows);
     count = cv.take<int>(4);
+    alpha = cv.take<float>(4);
     hc = cv.take<T>(capp * dp);
-    wp = pad_w ? cv.take<T>(vp * dp) : nullptr;
+    wp = pad_w ? cv.take<bf16>(vp * dp) : nullptr;
     losses = cv.take<float>(c.rows);
-    lse = cv.take<float>(c.rows);
+    norm = cv.take<float2>(c.rows);
     z = cv.take<float>(c.rows * c.k);
-    stats = c.grad_rows ? nullptr : cv.take<float2>(cap * blocks);
-    sums = c.smooth != 0 && !c.grad_rows ? cv.take<float>(cap * blocks) : nullptr;
-    slopes = c.grad_rows ? cv.take<RowSlope>(capp) : nullptr;
-    kept = grads ? static_cast<void*>(cv.take<T>(capp * vp)) : nullptr;
-    keptT = f32 && c.dw ? cv.take<T>(c.vocab * capp) : nullptr;
-    hcT = f32 && c.dw ? cv.take<T>(c.d * capp) : nullptr;
-    wT = f32 && c.dh ? cv.take<T>(c.d * vp) : nullptr;
+    caught = join ? cv.take<float>(cap * c.k) : nullptr;
+    stats = join || f32 ? cv.take<float2>(cap * blocks) : nullptr;
+    sums = c.smooth != 0 && join ? cv.take<float>(cap * blocks) : nullptr;
+    rows = RowsOut{grads && (f32 || c.grad_rows) ? cv.take<RowSlope>(capp) : nullptr,
+                   grads && (f32 || c.grad_rows) ? cv.take<float>(capp) : nullptr, nullptr};
+    kept = grads ? cv.take<T>(capp * vp) : nullptr;
+    hp = wpl = sp = wt = ah = nullptr;
+    eh = ew = es = ewt = eah = nullptr;
+    wpart = nullptr;
+    if (f32) {
+      hp = cv.take<sp16>(2 * capp * dp);
+      wpl = cv.take<sp16>(2 * c.vocab * dp);
+      eh = cv.take<int>(capp);
+      ew = cv.take<int>(c.vocab);
+    }
+    if (f32 && grads) {
+      rows.maxima = cv.take<unsigned>(vp + dp);
+      es = cv.take<int>(vp + dp);
+      eah = es + vp;
+      sp = cv.take<sp16>(2 * capp * vp);
+      if (c.dw) ah = cv.take<sp16>(2 * capp * dp);
+      if (c.dh) {
+        wt = cv.take<sp16>(2 * c.d * vp);
+        ewt = cv.take<int>(round_up(c.d, 8));
+        wpart = cv.take<unsigned>(round_up(c.d, 8) * absmax_col_parts(c.vocab));
+      }
+    }
     parts = c.dh ? grad_parts<T>(cap, c.d, vp, &part_tile) : 1;
+    part_len = (int)((vp / kPadK + parts - 1) / parts * kPadK);
     part = parts > 1 ? cv.take<float>(parts * cap * dp) : nullptr;
     acc = !f32 && c.dw && chunks(c) > 1 ? cv.take<float>(c.vocab * c.d) : nullptr;
   }
@@ -816,17 +1151,109 @@ size_t loss_ws_bytes(const Call& c) {
   return cv.used + 512;
 }
 
-// A product with the tile given (K-contiguous operands).
+// The logits' product: 256² or 128² tiles, both of 64-column wave tiles.
 template <typename T, class Epi>
-int launch_nt(const GemmArgs& g, const Epi& e, int batch, bool big, hipStream_t s, const char* name) {
-  PTO_REQUIRE(g.K % ring_k<T>() == 0 && g.ldp % (16 / sizeof(T)) == 0 && g.ldq % (16 / sizeof(T)) == 0 &&
-                  ((reinterpret_cast<uintptr_t>(g.P) | reinterpret_cast<uintptr_t>(g.Q)) & 15) == 0,
-              std::string(name) + ": operands not padded or not 16-byte aligned");
-  // a direct epilogue needs 64-column wave tiles: fp32's 128² tile, either bf16 tile
-  if (big || (IsDirect<Epi>::value && sizeof(T) == 4))
-    return launch_gemm_cfg<T, typename TileSet<T>::big, false>(g, e, batch, s, name);
-  if constexpr (!IsDirect<Epi>::value || sizeof(T) == 2) return launch_gemm_cfg<T, typename TileSet<T>::small, false>(g, e, batch, s, name);
-  return -1;
+int launch_logits(const ArgsOf<Operand<T>>& g, const Epi& e, hipStream_t s) {
+  typedef Operand<T> O;
+  const int64_t cus = device_cus();
+  auto rounds = [&](int64_t b) { return double(((g.M + b - 1) / b * ((g.N + b - 1) / b) + cus - 1) / cus) * b * b; };
+  if (rounds(256) < rounds(128) * TileSet<O>::kBigRate)
+    return launch_gemm_cfg<O, typename TileSet<O>::big, false>(g, e, 1, s, "loss_logits");
+  return launch_gemm_cfg<O, Tile<128, 128, 32, 2, 2>, false>(g, e, 1, s, "loss_logits");
+}
+
+// dH and dW of a chunk from its S.
+int chunk_gradients(const Call& c, const Ws<bf16>& w, const Chunk& ch, const bf16* W, int64_t ldw, bool first, bool last,
+                    hipStream_t s) {
+  bf16 *dh = static_cast<bf16*>(c.dh), *dw = static_cast<bf16*>(c.dw);
+  if (dh && ch.cap > 0) {
+    GemmArgs g{w.kept, w.vp, 0, W, ldw, 0, ch.cap, (int)c.d, (int)w.vp, 0, 0, nullptr};
+    if (w.parts > 1) {
+      g.K = w.part_len;
+      g.sP = w.part_len;
+      g.sQ = w.part_len * ldw;
+      const EpiPart e{{}, ch, w.part, w.dp, w.cap * w.dp, w.part_len, (int)w.vp};
+      if (launch_gemm_qn(g, e, w.parts, s, "loss_dhidden", w.part_tile)) return -1;
+      hipLaunchKernelGGL(join_parts_kernel<bf16>, dim3((unsigned)ch.cap), dim3(256), 0, s, ch, w.part, w.dp,
+                         w.cap * w.dp, w.parts, c.d, w.alpha, dh);
+      PTO_LAUNCHED("join_parts");
+    } else {
+      const EpiRows<bf16> e{{}, ch, dh, c.d, w.alpha};
+      if (launch_gemm_qn(g, e, 1, s, "loss_dhidden", w.part_tile)) return -1;
+    }
+  }
+  if (dw) {
+    const int k = (int)round_up(ch.cap, kPadK);
+    const GemmArgs g{w.kept, w.vp, 0, w.hc, w.dp, 0, (int)c.vocab, (int)c.d, k, 0, 0, nullptr};
+    const EpiWeight<bf16> e{{}, ch, w.acc, dw, c.d, first, last, w.alpha};
+    if (launch_gemm_qn<EpiWeight<bf16>, true>(g, e, 1, s, "loss_dweight")) return -1;
+  }
+  return 0;
+}
+
+int chunk_gradients(const Call& c, const Ws<float>& w, const Chunk& ch, const LossSpec& sp, const float* z, bool first,
+                    bool last, hipStream_t s) {
+  float *dh = static_cast<float*>(c.dh), *dw = static_cast<float*>(c.dw);
+  const int k = (int)round_up(ch.cap, kPadK);
+  if (ch.cap > 0) {
+    hipLaunchKernelGGL(column_max_kernel<true>, dim3((unsigned)((w.vp + 1023) / 1024), (unsigned)((ch.cap + 63) / 64)),
+                       dim3(256), 0, s, ch, w.kept, w.vp, (int)c.vocab, w.rows.slope, w.rows.a, w.rows.maxima);
+    PTO_LAUNCHED("column_max");
+    if (dw) {
+      hipLaunchKernelGGL(column_max_kernel<false>,
+                         dim3((unsigned)((w.dp + 1023) / 1024), (unsigned)((ch.cap + 63) / 64)), dim3(256), 0, s, ch,
+                         w.hc, w.dp, (int)c.d, w.rows.slope, w.rows.a, w.rows.maxima + w.vp);
+      PTO_LAUNCHED("column_max");
+    }
+    hipLaunchKernelGGL(exponents_kernel, dim3((unsigned)((w.vp + w.dp + 255) / 256)), dim3(256), 0, s, w.rows.maxima,
+                       w.vp + w.dp, w.es);
+    PTO_LAUNCHED("exponents");
+    hipLaunchKernelGGL(column_planes_kernel<true>, dim3((unsigned)k), dim3(256), 0, s, ch, w.kept, w.vp, (int)c.vocab,
+                       w.rows.slope, w.rows.a, w.es, w.sp, w.capp * w.vp, sp.k, w.t, z);
+    PTO_LAUNCHED("column_planes");
+  }
+  if (dh && ch.cap > 0) {
+    SplitPack p{};
+    p.in = static_cast<const float*>(c.w);
+    p.rows = c.vocab;
+    p.cols = c.d;
+    p.ld_in = c.ldw;
+    p.cpart = w.wpart;
+    p.nw = round_up(c.d, 8);
+    p.ec = w.ewt;
+    p.out_t = w.wt;
+    p.pl_t = c.d * w.vp;
+    p.ld_t = w.vp;
+    p.pre_r = w.es;
+    p.pre_mul = -1;
+    p.pre_off = kSplitTop;
+    if (launch_split_pack_max(p, 1, s, false)) return -1;
+    SplitArgs g{{w.sp, w.vp, 0, w.wt, w.vp, 0, ch.cap, (int)c.d, (int)w.vp}, w.capp * w.vp, c.d * w.vp};
+    if (w.parts > 1) {
+      g.K = w.part_len;
+      g.sP = w.part_len;
+      g.sQ = w.part_len;
+      const EpiPowers<EpiPart> e{{{}, ch, w.part, w.dp, w.cap * w.dp, w.part_len, (int)w.vp}, nullptr, w.ewt, -kSplitTop};
+      if (launch_gemm<sp16, false>(g, e, w.parts, s, "loss_dhidden")) return -1;
+      hipLaunchKernelGGL(join_parts_kernel<float>, dim3((unsigned)ch.cap), dim3(256), 0, s, ch, w.part, w.dp,
+                         w.cap * w.dp, w.parts, c.d, w.rows.a, dh);
+      PTO_LAUNCHED("join_parts");
+    } else {
+      const EpiPowers<EpiRows<float>> e{{{}, ch, dh, c.d, w.rows.a}, nullptr, w.ewt, -kSplitTop};
+      if (launch_gemm<sp16, false>(g, e, 1, s, "loss_dhidden")) return -1;
+    }
+  }
+  if (dw) {
+    if (ch.cap > 0) {
+      hipLaunchKernelGGL(column_planes_kernel<false>, dim3((unsigned)k), dim3(256), 0, s, ch, w.hc, w.dp, (int)c.d,
+                         w.rows.slope, w.rows.a, w.eah, w.ah, w.capp * w.dp, sp.k, w.t, z);
+      PTO_LAUNCHED("column_planes");
+    }
+    const SplitArgs g{{w.sp, w.vp, 0, w.ah, w.dp, 0, (int)c.vocab, (int)c.d, k}, w.capp * w.vp, w.capp * w.dp};
+    const EpiPowers<EpiWeight<float>> e{{{}, ch, dw, dw, c.d, first, last, nullptr}, w.es, w.eah, 0};
+    if (launch_gemm_qn<EpiPowers<EpiWeight<float>>, true, false, sp16>(g, e, 1, s, "loss_dweight")) return -1;
+  }
+  return 0;
 }
 
 template <typename T>
@@ -838,125 +1265,98 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
   const bool grads = c.dh || c.dw;
   const T* W = static_cast<const T*>(c.w);
   int64_t ldw = c.ldw;
-  if (c.rows == 0) {  // no row: loss and gradients of nothing
-    if (c.reduction && c.loss) {
-      hipLaunchKernelGGL(reduce_loss_kernel, dim3(1), dim3(1024), 0, s, w.losses, 0, w.count, 0, c.loss);
-      PTO_LAUNCHED("reduce_loss");
-    }
-  } else {
-    float* losses = c.reduction || !c.loss ? w.losses : c.loss;
-    if (c.y) {
-      hipLaunchKernelGGL(ce_targets_kernel, dim3((unsigned)((c.rows + 255) / 256)), dim3(256), 0, s, c.y, c.rows,
-                         c.vocab, c.ignore, (float)(1.0 - c.smooth), w.t, losses);
-    } else {
-      hipLaunchKernelGGL(kd_targets_kernel, dim3((unsigned)((c.rows + 3) / 4)), dim3(256), 0, s, c.teacher, c.index,
-                         c.rows, (int)c.k, c.vocab, (float)(1.0 / c.temp), w.t, losses);
-    }
-    PTO_LAUNCHED("loss_targets");
-    hipLaunchKernelGGL(list_rows_kernel, dim3(1), dim3(1024), 0, s, w.t.kept, c.rows, w.list, w.count);
-    PTO_LAUNCHED("list_rows");
-  }
-  if (w.pad_w) {
-    hipLaunchKernelGGL(pad_weight_kernel<T>, dim3((unsigned)((w.vp + 3) / 4)), dim3(256), 0, s, W, ldw, c.vocab, c.d,
-                       w.wp, w.dp, w.vp);
-    PTO_LAUNCHED("pad_weight");
-    W = w.wp;
-    ldw = w.dp;
-  }
-  if constexpr (f32) {
-    if (c.dh && launch_pack<T, T, float>(W, c.vocab, c.d, ldw, 0, nullptr, nullptr, 0, 0, w.wT, w.vp, 0, false, 1, s))
-      return -1;
-  }
-  float* lse = c.lse ? c.lse : w.lse;
+  float2* norm = c.norm ? reinterpret_cast<float2*>(c.norm) : w.norm;
   float* z = c.z ? c.z : w.z;
+  float* losses = c.reduction || !c.loss ? w.losses : c.loss;
   const float scale = (float)(1.4426950408889634 / c.temp);
-  const LossSpec sp{(float)(c.temp * c.temp), (float)(c.smooth / c.vocab), (float)c.zeta, (float)(1.0 / c.temp),
-                    (int)c.k, c.reduction};
+  const LossSpec sp{(float)(c.temp * c.temp), (float)(c.smooth / c.vocab), (float)c.zeta, (int)c.k};
+  if (c.kd && c.rows > 0) {
+    hipLaunchKernelGGL(kd_targets_kernel, dim3((unsigned)((c.rows + 3) / 4)), dim3(256), 0, s, c.teacher, c.index,
+                       c.rows, (int)c.k, c.vocab, (float)(1.0 / c.temp), w.t);
+    PTO_LAUNCHED("kd_targets");
+  }
+  hipLaunchKernelGGL(list_rows_kernel, dim3(1), dim3(1024), 0, s, c.kd ? nullptr : c.y, c.ignore, c.vocab, w.t, c.rows,
+                     w.list, w.count, c.grad_rows ? nullptr : losses, c.grad_rows, (float)c.temp, c.reduction == 1,
+                     w.alpha);
+  PTO_LAUNCHED("list_rows");
+  if (c.rows > 0) {
+    if constexpr (f32) {
+      hipLaunchKernelGGL(weight_planes_kernel, dim3((unsigned)((c.vocab + 3) / 4)), dim3(256), 0, s, W, ldw, c.vocab,
+                         c.d, w.wpl, w.dp, w.ew);
+      PTO_LAUNCHED("weight_planes");
+    } else if (w.pad_w) {
+      hipLaunchKernelGGL(pad_weight_kernel, dim3((unsigned)((w.vp + 3) / 4)), dim3(256), 0, s, W, ldw, c.vocab, c.d,
+                         w.wp, w.dp, w.vp);
+      PTO_LAUNCHED("pad_weight");
+      W = w.wp;
+      ldw = w.dp;
+    }
+  }
   const int64_t chunks = std::max<int64_t>(w.chunks(c), c.dw ? 1 : 0);  // no rows: dW is still written
   for (int64_t n = 0; n < chunks; ++n) {
     const Chunk ch{w.list, w.count, c.rows, (int)(n * w.cap), (int)std::min(w.cap, c.rows - n * w.cap)};
-    const int capp = (int)round_up(ch.cap, kPadK);
-    if (c.rows > 0) {
-      hipLaunchKernelGGL(gather_kernel<T>, dim3((unsigned)(capp / 4)), dim3(256), 0, s, ch, static_cast<const T*>(c.h),
-                         c.ldh, c.d, w.hc, w.dp, static_cast<T*>(c.dh));
-      PTO_LAUNCHED("gather");
-      GemmArgs g{w.hc, w.dp, 0, W, ldw, 0, ch.cap, (int)w.vp, (int)w.dp, 0, 0, nullptr};
-      const bool big = pick_tile<T, false>(ch.cap, w.vp, 1) == 1;
-      if (c.grad_rows) {
-        hipLaunchKernelGGL(row_slopes_kernel, dim3((unsigned)((capp + 255) / 256)), dim3(256), 0, s, ch, sp, w.t, z,
-                           lse, c.grad_rows, w.slopes);
-        PTO_LAUNCHED("row_slopes");
-        g.M = capp;
-        const EpiLogits<T, false, true> e{ch, (int)c.vocab, scale, nullptr, nullptr, w.blocks, w.kept, w.vp, w.slopes};
-        if (launch_nt<T>(g, e, 1, big, s, "loss_logits")) return -1;
-        hipLaunchKernelGGL(put_targets_kernel<T>, dim3((unsigned)ch.cap), dim3(64), 0, s, ch, sp, w.t, z, w.slopes,
-                           c.grad_rows, static_cast<T*>(w.kept), w.vp);
-        PTO_LAUNCHED("put_targets");
+    if (ch.cap > 0) {
+      const unsigned capp = (unsigned)round_up(ch.cap, kPadK);
+      GemmArgs base{w.hc, w.dp, 0, W, ldw, 0, ch.cap, (int)w.vp, (int)w.dp, 0, 0, nullptr};
+      ArgsOf<Operand<T>> g{base};
+      if constexpr (f32) {
+        hipLaunchKernelGGL(gather_planes_kernel, dim3(capp / 4), dim3(256), 0, s, ch, static_cast<const float*>(c.h),
+                           c.ldh, c.d, w.hc, w.dp, w.hp, w.capp * w.dp, w.eh, static_cast<float*>(c.dh), w.rows.maxima,
+                           grads ? w.vp + w.dp : 0);
+        g.P = w.hp;
+        g.Q = w.wpl;
+        g.ldq = w.dp;
+        g.pP = w.capp * w.dp;
+        g.pQ = c.vocab * w.dp;
       } else {
-        hipLaunchKernelGGL(dots_kernel<T>, dim3((unsigned)((ch.cap * c.k + 3) / 4)), dim3(256), 0, s, ch, w.hc, w.dp,
-                           static_cast<const T*>(c.w), c.ldw, c.d, (int)c.k, w.t, scale, z);
-        PTO_LAUNCHED("dots");
-        float* losses = c.reduction ? w.losses : c.loss;
-        if (grads) {
-          const EpiLogits<T, true, false> e{ch, (int)c.vocab, scale, w.stats, w.sums, w.blocks, w.kept, w.vp, nullptr};
-          if (launch_nt<T>(g, e, 1, big, s, "loss_logits")) return -1;
-          hipLaunchKernelGGL((finish_kernel<T, true>), dim3((unsigned)capp), dim3(256), 0, s, ch, w.stats, w.sums,
-                             w.blocks, sp, w.t, z, (int)c.vocab, w.kept, w.vp, losses, lse);
+        hipLaunchKernelGGL(gather_kernel, dim3(capp / 4), dim3(256), 0, s, ch, static_cast<const bf16*>(c.h), c.ldh,
+                           c.d, w.hc, w.dp, static_cast<bf16*>(c.dh));
+      }
+      PTO_LAUNCHED("gather");
+      if (c.kd) {
+        hipLaunchKernelGGL(mark_targets_kernel, dim3((unsigned)ch.cap), dim3(256), (unsigned)(w.blocks * 10), s, ch,
+                           w.blocks, (int)c.k, w.t);
+        PTO_LAUNCHED("mark_targets");
+      }
+      if (c.grad_rows) {
+        hipLaunchKernelGGL(row_slopes_kernel<T>, dim3(capp / 4), dim3(256), 0, s, ch, sp, w.t, z, norm, c.grad_rows,
+                           (float)c.temp, w.alpha, w.rows);
+        PTO_LAUNCHED("row_slopes");
+        if constexpr (f32) {
+          const EpiLogits<T, true, false> e{ch,      (int)c.vocab, scale, w.stats, nullptr, w.blocks, w.kept,
+                                            w.vp,    nullptr,      w.eh,  w.ew,    w.t,     sp.k,     nullptr};
+          if (launch_logits<T>(g, e, s)) return -1;
         } else {
-          const EpiLogits<T, false, false> e{ch,       (int)c.vocab, scale,   w.stats, w.sums,
-                                             w.blocks, nullptr,      w.vp,    nullptr};
-          if (launch_nt<T>(g, e, 1, big, s, "loss_logits")) return -1;
-          hipLaunchKernelGGL((finish_kernel<T, false>), dim3((unsigned)ch.cap), dim3(256), 0, s, ch, w.stats, w.sums,
-                             w.blocks, sp, w.t, z, (int)c.vocab, nullptr, w.vp, losses, lse);
+          g.M = (int)capp;
+          const EpiLogits<T, false, true> e{ch,   (int)c.vocab, scale,   nullptr, nullptr, w.blocks, w.kept,
+                                            w.vp, w.rows.slope, nullptr, nullptr, w.t,     sp.k,     nullptr};
+          if (launch_logits<T>(g, e, s)) return -1;
+          hipLaunchKernelGGL(put_targets_kernel, dim3((unsigned)ch.cap), dim3(64), 0, s, ch, sp.k, w.t, z, w.rows,
+                             w.kept, w.vp);
+          PTO_LAUNCHED("put_targets");
         }
+      } else {
+        auto logits = [&](auto keep) {
+          const EpiLogits<T, decltype(keep)::value, false> e{ch,     (int)c.vocab, scale, w.stats, w.sums,
+                                                             w.blocks, w.kept,     w.vp,  nullptr, w.eh,
+                                                             w.ew,   w.t,          sp.k,  w.caught};
+          return launch_logits<T>(g, e, s);
+        };
+        if (grads ? logits(std::true_type{}) : logits(std::false_type{})) return -1;
+        hipLaunchKernelGGL((grads ? finish_kernel<T, true> : finish_kernel<T, false>), dim3(capp), dim3(256), 0, s, ch,
+                           w.stats, w.sums, w.blocks, sp, w.t, w.caught, (int)c.vocab, reinterpret_cast<bf16*>(w.kept),
+                           w.vp, w.rows, w.alpha, losses, norm, z);
         PTO_LAUNCHED("finish");
       }
     }
-    const T* S = static_cast<const T*>(w.kept);
-    if (c.dh && c.rows > 0) {
-      const int len = (int)(round_up((w.vp / kPadK + w.parts - 1) / w.parts, 1) * kPadK);
-      GemmArgs g{S, w.vp, 0, f32 ? w.wT : W, f32 ? w.vp : ldw, 0, ch.cap, (int)c.d, (int)w.vp, 0, 0, nullptr};
-      if (w.parts > 1) {
-        g.K = len;
-        g.sP = len;
-        g.sQ = f32 ? len : len * ldw;
-        const EpiPart e{ch, w.part, w.dp, w.cap * w.dp, len, (int)w.vp};
-        if constexpr (f32) {
-          if (launch_nt<T>(g, e, w.parts, w.part_tile, s, "loss_dhidden")) return -1;
-        } else {
-          if (launch_gemm_qn(g, e, w.parts, s, "loss_dhidden", w.part_tile)) return -1;
-        }
-        hipLaunchKernelGGL(join_parts_kernel<T>, dim3((unsigned)ch.cap), dim3(256), 0, s, ch, w.part, w.dp,
-                           w.cap * w.dp, w.parts, c.d, static_cast<T*>(c.dh));
-        PTO_LAUNCHED("join_parts");
-      } else {
-        const EpiRows<T> e{ch, static_cast<T*>(c.dh), c.d};
-        if constexpr (f32) {
-          if (launch_nt<T>(g, e, 1, w.part_tile, s, "loss_dhidden")) return -1;
-        } else {
-          if (launch_gemm_qn(g, e, 1, s, "loss_dhidden", w.part_tile)) return -1;
-        }
-      }
-    }
-    if (c.dw) {
-      const bool first = n == 0, last = n == chunks - 1;
-      T* dw = static_cast<T*>(c.dw);
-      if constexpr (f32) {
-        if (launch_pack<T, T, float>(S, capp, c.vocab, w.vp, 0, nullptr, nullptr, 0, 0, w.keptT, w.capp, 0, false, 1,
-                                     s) ||
-            launch_pack<T, T, float>(w.hc, capp, c.d, w.dp, 0, nullptr, nullptr, 0, 0, w.hcT, w.capp, 0, false, 1, s))
-          return -1;
-        const GemmArgs g{w.keptT, w.capp, 0, w.hcT, w.capp, 0, (int)c.vocab, (int)c.d, capp, 0, 0, nullptr};
-        const EpiWeight<T> e{ch, dw, dw, c.d, first, last};
-        if (launch_nt<T>(g, e, 1, pick_tile<T, false>(c.vocab, c.d, 1) == 1, s, "loss_dweight")) return -1;
-      } else {
-        const GemmArgs g{S, w.vp, 0, w.hc, w.dp, 0, (int)c.vocab, (int)c.d, capp, 0, 0, nullptr};
-        const EpiWeight<T> e{ch, w.acc, dw, c.d, first, last};
-        if (launch_gemm_qn<EpiWeight<T>, true>(g, e, 1, s, "loss_dweight")) return -1;
-      }
+    const bool first = n == 0, last = n == chunks - 1;
+    if constexpr (f32) {
+      if (grads && chunk_gradients(c, w, ch, sp, z, first, last, s)) return -1;
+    } else {
+      if (grads && chunk_gradients(c, w, ch, W, ldw, first, last, s)) return -1;
     }
   }
-  if (c.rows > 0 && c.reduction && c.loss) {
+  if (c.reduction && c.loss) {
     hipLaunchKernelGGL(reduce_loss_kernel, dim3(1), dim3(1024), 0, s, w.losses, c.rows, w.count, c.reduction == 1,
                        c.loss);
     PTO_LAUNCHED("reduce_loss");
@@ -978,8 +1378,9 @@ int check(const Call& c, int dtype, void* ws, size_t ws_bytes) {
   PTO_REQUIRE(std::isfinite(c.zeta), n + ": z_loss must be finite");
   PTO_REQUIRE(c.w && (c.rows == 0 || (c.h && (c.y || (c.teacher && c.index)))), n + ": null operand");
   PTO_REQUIRE(c.grad_rows || c.loss || (c.rows == 0 && c.reduction == 0), n + ": null loss");
-  PTO_REQUIRE(!c.grad_rows || c.rows == 0 || (c.lse && c.z && (c.dh || c.dw)),
-              n + ": null lse, target logits or gradients of a backward call");
+  PTO_REQUIRE(!c.grad_rows || c.rows == 0 || (c.norm && c.z && (c.dh || c.dw)),
+              n + ": null normalisers, target logits or gradients of a backward call");
+  PTO_REQUIRE(!c.kd || c.vocab <= kMaxMarked, n + ": at most 393216 tokens");
   PTO_REQUIRE(c.grad_rows || c.reduction || !(c.dh || c.dw), n + ": gradients of losses per row need their gradients");
   PTO_REQUIRE((reinterpret_cast<uintptr_t>(c.w) & 15) == 0, n + ": weight must be 16-byte aligned");
   PTO_REQUIRE(ws || ws_bytes == 0, n + ": null workspace");
@@ -998,7 +1399,7 @@ int run(const Call& c, int dtype, void* ws, size_t ws_bytes, void* stream) {
 extern "C" {
 
 size_t pto_linear_loss_workspace_bytes(int dtype, int64_t rows, int64_t d, int64_t vocab, int64_t k, int64_t ldw,
-                                       double label_smoothing, int backward, int dhidden, int dweight,
+                                       double label_smoothing, int distillation, int backward, int dhidden, int dweight,
                                        int64_t chunk_bytes) {
   if (rows < 0 || d < 1 || vocab < 1 || k < 1) return 0;
   static const float one = 1.f;
@@ -1010,6 +1411,7 @@ size_t pto_linear_loss_workspace_bytes(int dtype, int64_t rows, int64_t d, int64
   c.k = k;
   c.ldw = ldw;
   c.smooth = label_smoothing;
+  c.kd = distillation != 0;
   c.grad_rows = backward ? &one : nullptr;
   c.dh = dhidden ? &some : nullptr;
   c.dw = dweight ? &some : nullptr;
@@ -1024,10 +1426,10 @@ size_t pto_linear_loss_workspace_bytes(int dtype, int64_t rows, int64_t d, int64
 int pto_linear_cross_entropy(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, const int64_t* targets,
                              int dtype, int64_t rows, int64_t d, int64_t vocab, int64_t ignore_index,
                              double label_smoothing, double z_loss, int reduction, const float* grad_rows, float* loss,
-                             float* lse, float* z, void* dhidden, void* dweight, int64_t chunk_bytes, void* workspace,
+                             float* norm, float* z, void* dhidden, void* dweight, int64_t chunk_bytes, void* workspace,
                              size_t ws_bytes, void* stream) {
-  const pto::Call c{hidden, ldh,  weight,         ldw,    targets,   ignore_index, nullptr, nullptr, rows,    d,
-                    vocab,  1,    1.0,            label_smoothing,   z_loss,       reduction, grad_rows, loss, lse,
+  const pto::Call c{hidden, ldh,  weight,         ldw,    false, targets,   ignore_index, nullptr, nullptr, rows,    d,
+                    vocab,  1,    1.0,            label_smoothing,   z_loss,       reduction, grad_rows, loss, norm,
                     z,      dhidden, dweight,     chunk_bytes, "linear_cross_entropy"};
   return pto::run(c, dtype, workspace, ws_bytes, stream);
 }
@@ -1035,10 +1437,10 @@ int pto_linear_cross_entropy(const void* hidden, int64_t ldh, const void* weight
 int pto_linear_distillation(const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                             const float* teacher_logits, const int64_t* teacher_index, int dtype, int64_t rows,
                             int64_t d, int64_t vocab, int64_t k, double temperature, int reduction,
-                            const float* grad_rows, float* loss, float* lse, float* z, void* dhidden, void* dweight,
+                            const float* grad_rows, float* loss, float* norm, float* z, void* dhidden, void* dweight,
                             int64_t chunk_bytes, void* workspace, size_t ws_bytes, void* stream) {
-  const pto::Call c{hidden, ldh, weight, ldw, nullptr, 0,   teacher_logits, teacher_index, rows, d,
-                    vocab,  k,   temperature, 0.0, 0.0, reduction, grad_rows, loss, lse,
+  const pto::Call c{hidden, ldh, weight, ldw, true, nullptr, 0,   teacher_logits, teacher_index, rows, d,
+                    vocab,  k,   temperature, 0.0, 0.0, reduction, grad_rows, loss, norm,
                     z,      dhidden, dweight, chunk_bytes, "linear_distillation"};
   return pto::run(c, dtype, workspace, ws_bytes, stream);
 }

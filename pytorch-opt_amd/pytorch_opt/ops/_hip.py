@@ -76,7 +76,7 @@ SIGNATURES = {
     "pto_shampoo_graft": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_i64, _c_dbl, _c_dbl, _c_dbl,
                                    _c_dbl, _c_ptr, _c_ptr, _c_size, _c_ptr]),
     "pto_linear_loss_workspace_bytes": (_c_size, [_c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_dbl, _c_int,
-                                                  _c_int, _c_int, _c_i64]),
+                                                  _c_int, _c_int, _c_int, _c_i64]),
     "pto_linear_cross_entropy": (_c_int, [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_int, _c_i64, _c_i64, _c_i64,
                                           _c_i64, _c_dbl, _c_dbl, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                                           _c_ptr, _c_i64, _c_ptr, _c_size, _c_ptr]),

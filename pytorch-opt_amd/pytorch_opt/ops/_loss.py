@@ -5,7 +5,7 @@ With a mean or sum the forward call also returns the gradients of hidden and
 weight, so the backward only multiplies them by the gradient of the loss (in
 place, and not at all where that is 1). They are handed out once; a second
 backward through a retained graph computes them again. With one loss per row
-the forward keeps lse and the targets' logits, and the backward computes the
+the forward keeps the normalisers and the targets' logits, and the backward computes the
 gradients under the rows' own.
 """
 
@@ -40,7 +40,7 @@ class _Call:
         self.backend, self.what, self.labels, self.k = backend, what, labels, k
         self.options, self.reduction = options, _REDUCTION_CODE[reduction]
 
-    def __call__(self, h, w, loss=None, lse=None, z=None, dh=None, dw=None, grad_rows=None):
+    def __call__(self, h, w, loss=None, norm=None, z=None, dh=None, dw=None, grad_rows=None):
         be, lib = self.backend, self.backend._lib
         code, (rows, d), vocab = _DTYPE_CODE[h.dtype], h.shape, w.shape[0]
         ldh = h.stride(0) if rows > 1 else d
@@ -48,13 +48,13 @@ class _Call:
         smoothing = self.options[1] if self.what == "linear_cross_entropy" else 0.0
         with torch.cuda.device(h.device):
             nbytes = lib.pto_linear_loss_workspace_bytes(code, rows, d, vocab, self.k, ldw, smoothing,
-                                                         int(grad_rows is not None), int(dh is not None),
+                                                         int(self.what == "linear_distillation"), int(grad_rows is not None), int(dh is not None),
                                                          int(dw is not None), be.LOSS_CHUNK_BYTES)
             ws = be._workspace(nbytes, h.device)
             sizes = (code, rows, d, vocab) if self.what == "linear_cross_entropy" else (code, rows, d, vocab, self.k)
             rc = getattr(lib, "pto_" + self.what)(
                 _ptr(h), ldh, _ptr(w), ldw, *(_ptr(t) for t in self.labels), *sizes, *self.options, self.reduction,
-                _ptr(grad_rows), _ptr(loss), _ptr(lse), _ptr(z), _ptr(dh), _ptr(dw), be.LOSS_CHUNK_BYTES, _ptr(ws),
+                _ptr(grad_rows), _ptr(loss), _ptr(norm), _ptr(z), _ptr(dh), _ptr(dw), be.LOSS_CHUNK_BYTES, _ptr(ws),
                 nbytes, be._stream(h.device))
         be._check(rc, self.what)
 
@@ -81,12 +81,12 @@ class _LinearLoss(torch.autograd.Function):
                 call(h, w, loss=loss)
             return loss
         loss = torch.empty(h.shape[0], dtype=torch.float32, device=h.device)
-        lse = z = None
+        norm = z = None
         if any(needs):
-            lse = torch.empty_like(loss)
+            norm = torch.empty(2 * h.shape[0], dtype=torch.float32, device=h.device)
             z = torch.empty(h.shape[0] * call.k, dtype=torch.float32, device=h.device)
-            ctx.save_for_backward(h, w, lse, z)
-        call(h, w, loss=loss, lse=lse, z=z)
+            ctx.save_for_backward(h, w, norm, z)
+        call(h, w, loss=loss, norm=norm, z=z)
         return loss
 
     @staticmethod
@@ -95,10 +95,10 @@ class _LinearLoss(torch.autograd.Function):
         call, be = ctx.call, ctx.call.backend
         grad = grad.to(torch.float32).contiguous()
         if not call.reduction:
-            h, w, lse, z = ctx.saved_tensors
+            h, w, norm, z = ctx.saved_tensors
             if h.shape[0] == 0:
                 return (*(torch.zeros_like(t) if n else None for t, n in zip((h, w), ctx.needs)), None, None)
-            dh, dw = call.gradients(h, w, ctx.needs, lse=lse, z=z, grad_rows=grad)
+            dh, dw = call.gradients(h, w, ctx.needs, norm=norm, z=z, grad_rows=grad)
             return dh, dw, None, None
         grads, ctx.grads = ctx.grads, None
         if grads is None:

@@ -504,7 +504,7 @@ def test_library_refusals():
                                    1 << 30, None)
     assert rc != 0 and b"temperature" in L.pto_last_error()
     assert L.pto_scale(None, 0, 5, a, None) != 0 and L.pto_scale(None, 0, 0, None, None) == 0
-    small = L.pto_linear_loss_workspace_bytes(2, 1, 2048, 32000, 1, 2048, 0.0, 0, 0, 0, 0)
+    small = L.pto_linear_loss_workspace_bytes(2, 1, 2048, 32000, 1, 2048, 0.0, 0, 0, 0, 0, 0)
     assert 0 < small < 1 << 20  # scoring one token keeps no logits
-    most = L.pto_linear_loss_workspace_bytes(2, 1 << 16, 4096, 128000, 1, 4096, 0.0, 0, 1, 1, 0)
+    most = L.pto_linear_loss_workspace_bytes(2, 1 << 16, 4096, 128000, 1, 4096, 0.0, 0, 0, 1, 1, 0)
     assert most < (5 << 30) + 4 * 128000 * 4096  # 2 GiB of logits, dW's sums, statistics
