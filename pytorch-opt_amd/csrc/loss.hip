@@ -162,7 +162,6 @@ __global__ void __launch_bounds__(1024) list_rows_kernel(const int64_t* __restri
   auto counts = [&](int64_t r) { return r < r1 && (y ? y[r] != ignore : t.kept[r] != 0); };
   int n = 0;
   float m = 0.f;
-#pragma unroll 4
   for (int64_t b = r0; b < r0 + per; b += 64) {
     const int64_t r = b + lane;
     const bool c = counts(r);
@@ -183,7 +182,6 @@ __global__ void __launch_bounds__(1024) list_rows_kernel(const int64_t* __restri
     m = fmaxf(m, big[o]);
   }
   int64_t no = total + min(rows, r0) - yes;
-#pragma unroll 4
   for (int64_t b = r0; b < r0 + per; b += 64) {
     const int64_t r = b + lane;
     const bool c = counts(r);
@@ -431,20 +429,32 @@ struct EpiLogits {
     const bool whole = wc0 + kCols <= vocab;  // false in the last block of a row at most
     RowSlope* const rs = reinterpret_cast<RowSlope*>(lds);
     constexpr int R = FM * 16;
-    unsigned long long* const bits = reinterpret_cast<unsigned long long*>(lds);  // one: the row's token
+    unsigned long long* const bits = reinterpret_cast<unsigned long long*>(lds);
     uint16_t* const before = reinterpret_cast<uint16_t*>(bits + R);
     int* const er = reinterpret_cast<int*>(before + R);
     int ec[4] = {0, 0, 0, 0};
+    // rows with a target in these columns, one bit each
+    unsigned long long hit[(R + 63) / 64] = {};
     if (targets) {
-      const int64_t b = wc0 / kCols;
-      for (int r = lane; r < R; r += 64) {
-        const int i = wr0 + r;
-        const bool live = i < g.M;
-        if (tg.one) {
-          bits[r] = live ? (unsigned)tg.one[ch.base + i] : ~0u;
-        } else {
-          bits[r] = live ? tg.bits[b * ch.cap + i] : 0;
-          before[r] = live ? tg.before[b * ch.cap + i] : 0;
+#pragma unroll
+      for (int q = 0; q < (R + 63) / 64; ++q) {
+        const int r = q * 64 + lane, i = wr0 + r;
+        unsigned long long word = 0;
+        int first = 0;
+        if (r < R && i < g.M) {
+          if (tg.one) {
+            const unsigned at = (unsigned)tg.one[ch.base + i] - wc0;  // -2: past every block
+            word = at < kCols ? 1ull << at : 0;
+          } else {
+            const int64_t at = (int64_t)(wc0 / kCols) * ch.cap + i;
+            word = tg.bits[at];
+            first = tg.before[at];
+          }
+        }
+        hit[q] = __ballot(word != 0);
+        if (r < R) {
+          bits[r] = word;
+          before[r] = (uint16_t)first;
         }
       }
     }
@@ -459,6 +469,27 @@ struct EpiLogits {
     }
     __builtin_amdgcn_s_waitcnt(PTO_LGKM0);
     __builtin_amdgcn_wave_barrier();
+    auto value = [&](int fm, int r, int k) {
+      const float v = acc[fm][k][r];
+      return sizeof(T) == 4 ? ldexpf(v, -er[fm * 16 + sub + r] - ec[k]) : v;
+    };
+    if (targets) {
+#pragma unroll
+      for (int fm = 0; fm < FM; ++fm) {
+        if (((hit[fm / 4] >> (fm % 4 * 16)) & 0xffff) == 0) continue;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int at = fm * 16 + sub + r;
+          const unsigned long long word = bits[at];
+          const unsigned mine = (unsigned)(word >> (4 * l)) & 15u;
+          if (mine == 0) continue;
+          int64_t to = (int64_t)(wr0 + at) * k + before[at] + __popcll(word & ((1ull << (4 * l)) - 1));
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (mine >> c & 1) targets[to++] = value(fm, r, c) * scale;
+        }
+      }
+    }
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
 #pragma unroll
@@ -467,12 +498,7 @@ struct EpiLogits {
         const bool live = i < g.M;
         float v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = acc[fm][k][r];
-        if (sizeof(T) == 4) {
-          const int e = er[fm * 16 + sub + r];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] = ldexpf(v[k], -e - ec[k]);
-        }
+        for (int k = 0; k < 4; ++k) v[k] = value(fm, r, k);
         if (SLOPE) {
           const RowSlope p = rs[fm * 16 + sub + r];
           float t[4];
@@ -489,7 +515,6 @@ struct EpiLogits {
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] = c0 + k < vocab ? v[k] : -INFINITY;
         }
-        if (targets) catch_targets(v, bits[fm * 16 + sub + r], before[fm * 16 + sub + r], i, wc0, l);
         const float m = max16(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
         const float ref = m == -INFINITY ? 0.f : m * scale;  // a block of nothing but -inf sums to 0
         float x[4], s = 0.f;
@@ -521,25 +546,6 @@ struct EpiLogits {
           }
         }
       }
-    }
-  }
-  // The targets among a lane's four columns of a row.
-  __device__ __forceinline__ void catch_targets(const float (&v)[4], unsigned long long word, int first, int64_t i,
-                                                int wc0, int l) const {
-    if (tg.one) {
-      const unsigned at = (unsigned)word - wc0;  // -2 and left-out rows: past every block
-      if (at < kCols && (int)(at >> 2) == l) {
-        const int c = at & 3;
-        targets[i] = (c == 0 ? v[0] : c == 1 ? v[1] : c == 2 ? v[2] : v[3]) * scale;
-      }
-      return;
-    }
-    const unsigned mine = (unsigned)(word >> (4 * l)) & 15u;
-    if (mine) {
-      int64_t to = i * k + first + __popcll(word & ((1ull << (4 * l)) - 1));
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (mine >> c & 1) targets[to++] = v[c] * scale;
     }
   }
   // (x/128 + 1)·65535, rounded, between 0 and 65535
