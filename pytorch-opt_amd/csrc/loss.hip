@@ -56,6 +56,7 @@ constexpr double kLn2 = 0.6931471805599453;
 // less, which fp32 does not hold as normal numbers either. fp32 inputs keep
 // fp32.
 constexpr float kOctaves = 128.f;
+constexpr float kNear = 0x1p-32f;  // least sum of exponentials of a row against a shared reference
 
 // Sparse targets. Cross entropy has one per row, by listed row: the token, or
 // -2 where it is outside the vocabulary, with the same share in every row.
@@ -389,6 +390,16 @@ __device__ __forceinline__ float sum16(float v) {
   return v + dpp<0x140>(v);
 }
 
+// Sums of four values over 16 lanes each: lane l gets the sum of v[l & 3].
+__device__ __forceinline__ float sum_rows(const float (&v)[4], int l) {
+  const bool odd = l & 1, up = l & 2;
+  const float a = (odd ? v[1] : v[0]) + dpp<0xB1>(odd ? v[0] : v[1]);
+  const float b = (odd ? v[3] : v[2]) + dpp<0xB1>(odd ? v[2] : v[3]);
+  float s = (up ? b : a) + dpp<0x4E>(up ? a : b);
+  s += dpp<0x124>(s);  // row_ror 4
+  return s + dpp<0x128>(s);  // row_ror 8
+}
+
 // What a row's slopes need besides its logits t (in log2): S = pa·2^(t − m) + pu.
 struct RowSlope {
   float m, pa, pu;
@@ -490,6 +501,70 @@ struct EpiLogits {
         }
       }
     }
+    if constexpr (SLOPE) {
+#pragma unroll
+      for (int fm = 0; fm < FM; ++fm)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = wr0 + fm * 16 + sub + r;
+          const RowSlope p = rs[fm * 16 + sub + r];
+          float t[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            t[k] = fmaf(p.pa, pow2(fmaf(value(fm, r, k), scale, -p.m)), p.pu);
+            if (!whole) t[k] = c0 + k < vocab ? t[k] : 0.f;
+          }
+          if (i < g.M) st4(static_cast<T*>(kept) + i * ld + c0, t);
+        }
+      return;
+    }
+    // One reference for all of the wave's values: 0 or the largest. Kept logits
+    // and exponentials have the same relative precision however far below it
+    // they lie, so it serves every row whose own maximum is at most 2^kNear
+    // below; then a maximum per row (8 lane exchanges for each, half the
+    // epilogue's instructions) is not needed.
+    if (whole) {
+      // the order of non-negative floats is that of their bits; what is not a
+      // number is above them all
+      int top = 0;
+#pragma unroll
+      for (int fm = 0; fm < FM; ++fm)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = max(top, __float_as_int(value(fm, r, k)));
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
+      const float ref = __int_as_float(__builtin_amdgcn_readfirstlane(top)) * scale;
+      float least = INFINITY;
+      if (ref < INFINITY) {
+#pragma unroll
+        for (int fm = 0; fm < FM; ++fm) {
+          const int i0 = wr0 + fm * 16 + sub;
+          float s[4], z[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = value(fm, r, k);
+            s[r] = (pow2(fmaf(v[0], scale, -ref)) + pow2(fmaf(v[1], scale, -ref))) +
+                   (pow2(fmaf(v[2], scale, -ref)) + pow2(fmaf(v[3], scale, -ref)));
+            if (sums) z[r] = (v[0] + v[1]) + (v[2] + v[3]);
+            if (KEEP && i0 + r < g.M) keep(i0 + r, c0, v, ref);
+          }
+          // lane l: the sum of row r = l & 3
+          const float sum = sum_rows(s, l);
+          least = fminf(least, sum);
+          const bool mine = (l & 12) == 0 && i0 + (l & 3) < g.M;
+          if (mine) stats[(i0 + (l & 3)) * blocks + wc0 / kCols] = make_float2(ref, sum);
+          if (sums) {
+            const float zs = sum_rows(z, l) * scale;
+            if (mine) sums[(i0 + (l & 3)) * blocks + wc0 / kCols] = zs;
+          }
+        }
+        if (!__any(!(least >= kNear))) return;
+      }
+    }
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
 #pragma unroll
@@ -498,31 +573,15 @@ struct EpiLogits {
         const bool live = i < g.M;
         float v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = value(fm, r, k);
-        if (SLOPE) {
-          const RowSlope p = rs[fm * 16 + sub + r];
-          float t[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) t[k] = fmaf(p.pa, pow2(fmaf(v[k], scale, -p.m)), p.pu);
-          if (!whole) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) t[k] = c0 + k < vocab ? t[k] : 0.f;
-          }
-          if (live) st4(static_cast<T*>(kept) + i * ld + c0, t);
-          continue;
-        }
-        if (!whole) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] = c0 + k < vocab ? v[k] : -INFINITY;
+        for (int k = 0; k < 4; ++k) {
+          v[k] = value(fm, r, k);
+          if (!whole) v[k] = c0 + k < vocab ? v[k] : -INFINITY;
         }
         const float m = max16(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
         const float ref = m == -INFINITY ? 0.f : m * scale;  // a block of nothing but -inf sums to 0
-        float x[4], s = 0.f;
+        float s = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          x[k] = fmaf(v[k], scale, -ref);
-          s += pow2(x[k]);
-        }
+        for (int k = 0; k < 4; ++k) s += pow2(fmaf(v[k], scale, -ref));
         s = sum16(s);
         if (live && l == 0) stats[i * blocks + wc0 / kCols] = make_float2(ref, s);
         if (sums) {
@@ -532,26 +591,23 @@ struct EpiLogits {
           z = sum16(z) * scale;
           if (live && l == 0) sums[i * blocks + wc0 / kCols] = z;
         }
-        if (KEEP && live) {
-          if constexpr (sizeof(T) == 2) {
-            uint2 u;
-            u.x = encode(x[0], x[1]);
-            u.y = encode(x[2], x[3]);
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(kept) + i * ld + c0) = u;
-          } else {
-            float t[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) t[k] = v[k] * scale;
-            st4(static_cast<float*>(kept) + i * ld + c0, t);
-          }
-        }
+        if (KEEP && live) keep(i, c0, v, ref);
       }
     }
   }
-  // (x/128 + 1)·65535, rounded, between 0 and 65535
-  __device__ __forceinline__ static unsigned encode(float a, float b) {
-    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(fmaf(a, 1.f / kOctaves, 1.f),
-                                                                        fmaf(b, 1.f / kOctaves, 1.f)));
+  // Four columns of a row, kept.
+  __device__ __forceinline__ void keep(int64_t i, int c0, const float (&v)[4], float ref) const {
+    if constexpr (sizeof(T) == 2) {
+      // 1 + (t − ref)/128 of 65535, rounded, between 0 and 65535
+      const float f = scale / kOctaves, o = fmaf(-ref, 1.f / kOctaves, 1.f);
+      auto two = [&](float a, float b) {
+        return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(fmaf(a, f, o), fmaf(b, f, o)));
+      };
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(kept) + i * ld + c0) = make_uint2(two(v[0], v[1]), two(v[2], v[3]));
+    } else {
+      const float t[4] = {v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale};
+      st4(static_cast<float*>(kept) + i * ld + c0, t);
+    }
   }
   template <typename U>
   __device__ __forceinline__ static void st4(U* p, const float (&t)[4]) {
@@ -642,7 +698,7 @@ __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __r
   __shared__ float red[4][4];
   float m = -INFINITY;
   for (int64_t c = tid; c < blocks; c += 256)
-    if (st[c].y != 0.f) m = fmaxf(m, st[c].x);
+    if (st[c].y != 0.f) m = fmaxf(m, st[c].x + log2f(st[c].y));
   m = wave_max(m);
   if (lane == 0) red[0][w] = m;
   __syncthreads();
