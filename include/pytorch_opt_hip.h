@@ -297,8 +297,8 @@ int pto_linear_distillation(const void* hidden, int64_t ldh, const void* weight,
                             int64_t d, int64_t vocab, int64_t k, double temperature, int reduction,
                             const float* grad_rows, float* loss, float* norm, float* z, void* dhidden, void* dweight,
                             int64_t chunk_bytes, void* workspace, size_t ws_bytes, void* stream);
-/* x[0..n) *= factor[0] (device pointer) in place, nothing read where it is 1. */
-int pto_scale(void* x, int dtype, int64_t n, const float* factor, void* stream);
+/* x[0..n) and y[0..m) *= factor[0] (device pointer) in place, nothing read where it is 1. */
+int pto_scale_pair(void* x, int64_t n, void* y, int64_t m, int dtype, const float* factor, void* stream);
 
 /*
  * Kernel timing with HIP events. The reference has no counterpart (its

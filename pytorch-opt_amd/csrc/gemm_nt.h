@@ -377,12 +377,21 @@ struct HasSkip<E, std::void_t<decltype(std::declval<const E&>().skip(0, false))>
 //       shorten g.M and g.K (whole rings of K tiles) for the tile, from counts
 //       that only the device knows; false: the tile has no work (the
 //       workgroup exits). Every wave gets the same answer.
+//   `int work(const GemmArgs& g, ...) const` and `bool take(GemmArgs& g, int
+//       logical, int& ti, int& tj)`: the number of workgroups that have work (the
+//       launch has at least as many; the rest exit), and the tile of one of them,
+//       with g.P, g.Q and g.K moved to a part of K.
 //   `int q_rows() const`: rows of a K-contiguous Q that exist, where N
 //       counts the padded columns of the output (the rest re-read the last).
 template <class E, class = void>
 struct HasAdjust : std::false_type {};
 template <class E>
 struct HasAdjust<E, std::void_t<decltype(std::declval<const E&>().adjust(std::declval<GemmArgs&>(), 0, 0, 0))>>
+    : std::true_type {};
+template <class E, class = void>
+struct HasWork : std::false_type {};
+template <class E>
+struct HasWork<E, std::void_t<decltype(std::declval<const E&>().work(std::declval<const GemmArgs&>()))>>
     : std::true_type {};
 template <class E, class = void>
 struct HasQRows : std::false_type {};
@@ -728,14 +737,23 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_nt_kernel(Args g, Epi epi) {
   const int kg = KG == 1 ? 0 : wave / NWG, wl = wave - kg * NWG;  // K group, wave in the group
   const int wm = wl / Cfg::WN, wn = wl % Cfg::WN;
   const int ntile = gridDim.x;  // tiles per matrix
-  const int logical = xcd_remap(blockIdx.y * ntile + blockIdx.x, ntile * gridDim.y, g.cus);
-  const int b = logical / ntile;
+  int logical, b, ti, tj;
+  if constexpr (HasWork<Epi>::value) {
+    const int work = epi.work(g);
+    if ((int)blockIdx.x >= work) return;
+    logical = xcd_remap(blockIdx.x, work, g.cus);
+    b = 0;
+    if (!epi.take(g, logical, ti, tj)) return;
+  } else {
+    logical = xcd_remap(blockIdx.y * ntile + blockIdx.x, ntile * gridDim.y, g.cus);
+    b = logical / ntile;
+  }
   if (g.guard != nullptr && g.guard[(int64_t)b * g.guard_stride] != 0) return;
   if constexpr (HasSkip<Epi>::value) {
     if (epi.skip(b, logical == b * ntile)) return;
   }
-  int ti, tj;
-  if (UPPER && gridDim.y == 1 && g.tiles_n <= kUpperOrderMaxT && ntile == g.tiles_n * (g.tiles_n + 1) / 2 &&
+  if constexpr (HasWork<Epi>::value) {
+  } else if (UPPER && gridDim.y == 1 && g.tiles_n <= kUpperOrderMaxT && ntile == g.tiles_n * (g.tiles_n + 1) / 2 &&
       ntile <= g.cus) {
     // one round of one matrix: each XCD's contiguous range of logical ids
     // is a set of upper tiles chosen to read few operand panels

@@ -163,12 +163,18 @@ __global__ void __launch_bounds__(1024) list_rows_kernel(const int64_t* __restri
   auto counts = [&](int64_t r) { return r < r1 && (y ? y[r] != ignore : t.kept[r] != 0); };
   int n = 0;
   float m = 0.f;
-  for (int64_t b = r0; b < r0 + per; b += 64) {
-    const int64_t r = b + lane;
-    const bool c = counts(r);
-    n += __popcll(__ballot(c));
-    if (weights && c && fabsf(weights[r]) < INFINITY) m = fmaxf(m, fabsf(weights[r]));
-    if (losses && r < r1) losses[r] = 0.f;
+  // eight loads in flight
+  for (int64_t b = r0; b < r0 + per; b += 512) {
+    bool c[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) c[q] = counts(b + 64 * q + lane);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int64_t r = b + 64 * q + lane;
+      n += __popcll(__ballot(c[q]));
+      if (weights && c[q] && fabsf(weights[r]) < INFINITY) m = fmaxf(m, fabsf(weights[r]));
+      if (losses && r < r1) losses[r] = 0.f;
+    }
   }
   m = wave_max(m);
   if (lane == 0) {
@@ -183,20 +189,29 @@ __global__ void __launch_bounds__(1024) list_rows_kernel(const int64_t* __restri
     m = fmaxf(m, big[o]);
   }
   int64_t no = total + min(rows, r0) - yes;
-  for (int64_t b = r0; b < r0 + per; b += 64) {
-    const int64_t r = b + lane;
-    const bool c = counts(r);
-    const unsigned long long mask = __ballot(c), before = (1ull << lane) - 1;
-    const int at = __popcll(mask & before);
-    if (c) {
-      list[yes + at] = (int)r;
-      if (y) t.one[yes + at] = y[r] >= 0 && y[r] < vocab ? (int)y[r] : -2;
-    } else if (r < r1) {
-      list[no + lane - at] = (int)r;
+  for (int64_t b = r0; b < r0 + per; b += 512) {
+    bool c[8];
+    int64_t id[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int64_t r = b + 64 * q + lane;
+      c[q] = counts(r);
+      id[q] = y && r < r1 ? y[r] : 0;
     }
-    const int here = __popcll(mask);
-    yes += here;
-    no += 64 - here;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int64_t r = b + 64 * q + lane;
+      const unsigned long long mask = __ballot(c[q]);
+      const int at = __popcll(mask & ((1ull << lane) - 1)), here = __popcll(mask);
+      if (c[q]) {
+        list[yes + at] = (int)r;
+        if (y) t.one[yes + at] = id[q] >= 0 && id[q] < vocab ? (int)id[q] : -2;
+      } else if (r < r1) {
+        list[no + lane - at] = (int)r;
+      }
+      yes += here;
+      no += 64 - here;
+    }
   }
   if (threadIdx.x == 0) {
     count[0] = total;
@@ -210,7 +225,8 @@ struct Chunk {
   const int* count;
   int64_t rows;  // of the call
   int base, cap;  // first listed row, most rows
-  __device__ __forceinline__ int live() const { return max(0, min(cap, count[0] - base)); }
+  // count null: all of them
+  __device__ __forceinline__ int live() const { return count ? max(0, min(cap, count[0] - base)) : cap; }
   // rows that products reading them along K see: zero rows up to a multiple of kPadK
   __device__ __forceinline__ int padded() const { return (live() + kPadK - 1) / kPadK * kPadK; }
 };
@@ -323,18 +339,41 @@ __global__ void __launch_bounds__(256) pad_weight_kernel(const bf16* __restrict_
   copy_row(w + min(r, vocab - 1) * ldw, r < vocab ? d : 0, out + r * ldo, ldo, threadIdx.x & 63);
 }
 
+// Four values of a row of n (the rest 0).
+__device__ __forceinline__ void load_columns(const float* p, int n, float (&v)[4]) {
+  uint4 u = make_uint4(0, 0, 0, 0);
+  if (n >= 4) {
+    u = ld16(p);
+  } else {
+    if (n > 0) u.x = __float_as_uint(p[0]);
+    if (n > 1) u.y = __float_as_uint(p[1]);
+    if (n > 2) u.z = __float_as_uint(p[2]);
+  }
+  v[0] = __uint_as_float(u.x);
+  v[1] = __uint_as_float(u.y);
+  v[2] = __uint_as_float(u.z);
+  v[3] = __uint_as_float(u.w);
+}
 // A row of n floats as split planes (padded to ld, pl elements apart) with the
 // exponent of its largest finite value, one wave; copy: also as it is.
 __device__ __forceinline__ void row_planes(const float* __restrict__ src, int64_t n, sp16* __restrict__ dst, int64_t pl,
                                            int64_t ld, int* __restrict__ exponent, float* __restrict__ copy, int lane) {
   float m = 0.f;
-  for (int64_t c = lane; c < n; c += 64) m = fabsf(src[c]) < INFINITY ? fmaxf(m, fabsf(src[c])) : m;
+#pragma unroll 4
+  for (int64_t c = lane * 4; c < n; c += 256) {
+    float v[4];
+    load_columns(src + c, (int)(n - c), v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = fabsf(v[k]) < INFINITY ? fmaxf(m, fabsf(v[k])) : m;
+  }
   const int e = split_exp(wave_max(m));
   if (lane == 0) *exponent = e;
   for (int64_t c = lane * 8; c < ld; c += 512) {
-    float v[8];
+    float lo[4], hi[4], v[8];
+    load_columns(src + c, (int)(n - c), lo);
+    load_columns(src + c + 4, (int)(n - c) - 4, hi);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = c + k < n ? src[c + k] : 0.f;
+    for (int k = 0; k < 8; ++k) v[k] = k < 4 ? lo[k & 3] : hi[k & 3];
     if (copy) st8<float, float>(copy + c, v, 0, 8);
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = ldexpf(v[k], e);
@@ -822,22 +861,22 @@ __global__ void __launch_bounds__(1024) reduce_loss_kernel(const float* __restri
 // fp32: S/a and a·H as split planes for the gradients' products. dW sums over
 // the rows, so a column of each has an exponent of its own, from its largest
 // value: tokens that are unlikely in every row keep their bits. dH sums over
-// the vocabulary, with the columns' exponents taken out of W's rows
-// (launch_split_pack_max); a, which may differ by rows, multiplies its result.
+// the vocabulary, with the columns' exponents taken out of W's rows (undo); a,
+// which may differ by rows, multiplies its result.
 
 // Largest values of 1024 columns over 64 rows: of S/a (EXP, x = the logits) or
 // of a·x.
 template <bool EXP>
-__global__ void __launch_bounds__(256) column_max_kernel(Chunk ch, const float* __restrict__ x, int64_t ld, int cols,
+__global__ void __launch_bounds__(256) column_max_kernel(Chunk ch, const float* __restrict__ x, int64_t ld, int rows, int cols,
                                                          const RowSlope* __restrict__ slope,
                                                          const float* __restrict__ a, unsigned* __restrict__ maxima) {
-  const int c = (blockIdx.x * 256 + threadIdx.x) * 4, r0 = blockIdx.y * 64, r1 = min(r0 + 64, ch.live());
+  const int c = (blockIdx.x * 256 + threadIdx.x) * 4, r0 = blockIdx.y * 64, r1 = min(r0 + 64, min(rows, ch.live()));
   if (c >= cols) return;
   float m[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+#pragma unroll 8
   for (int i = r0; i < r1; ++i) {
-    const float4 t = *reinterpret_cast<const float4*>(x + i * ld + c);
-    const float v[4] = {t.x, t.y, t.z, t.w};
+    float v[4];
+    load_columns(x + i * ld + c, cols - c, v);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float w = fabsf(EXP ? fmaf(slope[i].pa, pow2(v[k] - slope[i].m), slope[i].pu) : a[i] * v[k]);
@@ -849,36 +888,34 @@ __global__ void __launch_bounds__(256) column_max_kernel(Chunk ch, const float* 
     if (c + k < cols && r0 < r1) atomicMax(&maxima[c + k], __float_as_uint(m[k]));
 }
 __global__ void __launch_bounds__(256) exponents_kernel(const unsigned* __restrict__ maxima, int64_t n,
-                                                        int* __restrict__ e) {
+                                                        int* __restrict__ e, float* __restrict__ undo) {
   const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c < n) e[c] = split_exp(__uint_as_float(maxima[c]));
+  if (c >= n) return;
+  e[c] = split_exp(__uint_as_float(maxima[c]));
+  if (undo) undo[c] = ldexpf(1.f, -e[c]);
 }
 // The planes, one workgroup per row; pad rows and columns 0.
 template <bool EXP>
-__global__ void __launch_bounds__(256) column_planes_kernel(Chunk ch, const float* __restrict__ x, int64_t ld, int cols,
-                                                            const RowSlope* __restrict__ slope,
+__global__ void __launch_bounds__(256) column_planes_kernel(Chunk ch, const float* __restrict__ x, int64_t ld, int rows,
+                                                            int cols, const RowSlope* __restrict__ slope,
                                                             const float* __restrict__ a, const int* __restrict__ ec,
-                                                            sp16* __restrict__ out, int64_t pl, int k, Targets tg,
+                                                            sp16* __restrict__ out, int64_t ldo, int64_t pl, int k,
+                                                            Targets tg,
                                                             const float* __restrict__ z) {
   const int i = blockIdx.x, tid = threadIdx.x;
-  if (i >= ch.padded()) return;
+  if (i >= min(rows, ch.padded())) return;
   const bool live = i < ch.live();
-  sp16* o = out + i * ld;
+  sp16* o = out + i * ldo;
   const RowSlope rs = EXP && live ? slope[i] : RowSlope{0.f, 0.f, 0.f};
   const float ai = !EXP && live ? a[i] : 0.f;
-  for (int64_t c = tid * 8; c < ld; c += 2048) {
-    float v[8];
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const float4 t = live ? *reinterpret_cast<const float4*>(x + i * ld + c + 4 * q) : make_float4(0, 0, 0, 0);
-      v[4 * q] = t.x;
-      v[4 * q + 1] = t.y;
-      v[4 * q + 2] = t.z;
-      v[4 * q + 3] = t.w;
-    }
+  for (int64_t c = tid * 8; c < ldo; c += 2048) {
+    float lo[4], hi[4], v[8];
+    load_columns(x + i * ld + c, live ? cols - (int)c : 0, lo);
+    load_columns(x + i * ld + c + 4, live ? cols - (int)c - 4 : 0, hi);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float w = EXP ? fmaf(rs.pa, pow2(v[k] - rs.m), rs.pu) : ai * v[k];
+      const float y = k < 4 ? lo[k & 3] : hi[k & 3];
+      const float w = EXP ? fmaf(rs.pa, pow2(y - rs.m), rs.pu) : ai * y;
       v[k] = live && c + k < cols ? ldexpf(w, ec[c + k]) : 0.f;
     }
     const Split8 s = split8(v);
@@ -903,17 +940,12 @@ __global__ void __launch_bounds__(256) column_planes_kernel(Chunk ch, const floa
 
 // ------------------------------------------------------------ gradients
 
-// What the three epilogues below share: no transposed pass, nothing read early.
+// What a tile's values become (EpiSplit drives them): adjust as in gemm_nt.h,
+// load what an output run needs, put it.
 struct EpiPlain {
   typedef float S;
   typedef NoPre Pre;
-  typedef NoPre PreT;
-  static constexpr bool kVoIsV = true;
-  __device__ __forceinline__ bool has_t() const { return false; }
   __device__ __forceinline__ void load(int, int, int, int, int, Pre&) const {}
-  __device__ __forceinline__ void load_t(int, int, int, int, PreT&) const {}
-  __device__ __forceinline__ void put_t(int, int, int, const S*, int, const PreT&) const {}
-  __device__ __forceinline__ void finish(int) const {}
 };
 
 // dH: rows of the chunk to their places, times what S is without: alpha, or
@@ -936,38 +968,6 @@ struct EpiRows : EpiPlain {
     st8<T, S>(dst + ch.list[ch.base + i] * ld + j0, w, kbeg, n);
   }
 };
-
-// dH of few rows: the vocabulary split over the batch index, partial sums to
-// the workspace.
-struct EpiPart : EpiPlain {
-  Chunk ch;
-  float* dst;
-  int64_t ld, sd;
-  int len, total;  // K of a slice, of all
-  __device__ __forceinline__ bool adjust(GemmArgs& g, int b, int row0, int) const {
-    g.M = ch.live();
-    g.K = max(0, min(len, total - b * len));
-    return row0 < g.M;
-  }
-  __device__ __forceinline__ void put(int b, int i, int j0, const S* v, int kbeg, int n, const Pre&, S*) const {
-    st8<float, S>(dst + b * sd + i * ld + j0, v, kbeg, n);
-  }
-};
-template <typename T>
-__global__ void __launch_bounds__(256) join_parts_kernel(Chunk ch, const float* __restrict__ part, int64_t ld,
-                                                         int64_t sd, int parts, int64_t d, const float* __restrict__ a,
-                                                         T* __restrict__ dst) {
-  const int i = blockIdx.x;
-  if (i >= ch.live()) return;
-  const float f = a[sizeof(T) == 4 ? i : 0];
-  T* row = dst + ch.list[ch.base + i] * d;
-  for (int64_t c = threadIdx.x; c < d; c += 256) {
-    float s = 0.f;
-#pragma unroll 8
-    for (int p = 0; p < parts; ++p) s += part[p * sd + i * ld + c];
-    row[c] = convert<T>(s * f);
-  }
-}
 
 // dW over the chunks of rows: acc = v (first), acc + v, and out = acc + v,
 // times alpha (bf16) and rounded (last); acc is out where the chunk is the only one or out is fp32.
@@ -1012,25 +1012,18 @@ struct EpiWeight : EpiPlain {
 // One of them over split operands: the powers of two of the rows (er, or none)
 // and columns taken out first.
 template <class In>
-struct EpiPowers {
-  typedef float S;
+struct EpiPowers : EpiPlain {
   typedef typename In::Pre Pre;
-  typedef NoPre PreT;
-  static constexpr bool kVoIsV = true;
   In in;
   const int *er, *ec;
   int off;
-  __device__ __forceinline__ bool has_t() const { return false; }
   __device__ __forceinline__ bool adjust(GemmArgs& g, int b, int row0, int col0) const {
     return in.adjust(g, b, row0, col0);
   }
-  __device__ __forceinline__ void load(int b, int i, int j0, int kbeg, int n, Pre& p, bool) const {
+  __device__ __forceinline__ void load(int b, int i, int j0, int kbeg, int n, Pre& p) const {
     in.load(b, i, j0, kbeg, n, p);
   }
-  __device__ __forceinline__ void load_t(int, int, int, int, PreT&, bool) const {}
-  __device__ __forceinline__ void put_t(int, int, int, const S*, int, const PreT&, bool) const {}
-  __device__ __forceinline__ void finish(int) const {}
-  __device__ __forceinline__ void put(int b, int i, int j0, const S* v, int kbeg, int n, const Pre& p, S*, bool) const {
+  __device__ __forceinline__ void put(int b, int i, int j0, const S* v, int kbeg, int n, const Pre& p, S*) const {
     S w[8], drop[8];
     const int e = off - (er ? er[i] : 0);
 #pragma unroll
@@ -1039,25 +1032,149 @@ struct EpiPowers {
   }
 };
 
-// x *= s[0] in place, nothing where s[0] is 1 (the gradient of a loss that is
-// itself differentiated).
+// Parts of K for the tiles that whole rounds of the CUs leave over: as many as
+// end soonest, with `unit` us for kPadK of K of a tile on one CU and the
+// partial tiles' way to memory and back (`area` elements) against it. How many
+// tiles there are only the device knows (rows left out), so the choice is made
+// there, by every workgroup alike.
+struct Parts {
+  int full, rest, parts;  // tiles in whole rounds, tiles left over, parts of each of those
+  float time;
+};
+constexpr int kMostParts = 16;
+__host__ __device__ inline Parts split_parts(int tiles, int units, int cus, float unit, int area, int most) {
+  Parts s;
+  s.full = tiles / cus * cus;
+  s.rest = tiles - s.full;
+  s.parts = 1;
+  s.time = s.rest > 0 ? units * unit : 0.f;
+  for (int p = 2; p <= most && p <= units && s.rest > 0 && s.rest * p <= 2 * cus; ++p) {
+    const float t = (float)((s.rest * p + cus - 1) / cus * ((units + p - 1) / p)) * unit + 7.f +
+                    (float)s.rest * p * area * (8.f / 4.5e6f);
+    if (t < s.time) {
+      s.time = t;
+      s.parts = p;
+    }
+  }
+  return s;
+}
+
+// Any of them, with the tiles of the last round in parts: partial tiles to the
+// workspace, joined by join_parts_kernel.
+template <class In, class Cfg, bool QN, bool PT, typename T>
+struct EpiSplit {
+  typedef float S;
+  typedef typename In::Pre Pre;
+  typedef NoPre PreT;
+  static constexpr bool kVoIsV = true;
+  static constexpr int BM = Cfg::BM, BN = Cfg::BN;
+  In in;
+  float* part;
+  float unit;
+  int most, cus;
+  int slot = -1, row0 = 0, col0 = 0;
+  struct Plan {
+    Parts s;
+    int tm, tn, units;
+  };
+  __device__ __forceinline__ bool plan(GemmArgs& g, Plan& p) const {
+    if (!in.adjust(g, 0, 0, 0)) return false;
+    p.tm = (g.M + BM - 1) / BM;
+    p.tn = (g.N + BN - 1) / BN;
+    p.units = g.K / kPadK;
+    p.s = split_parts(p.tm * p.tn, p.units, cus, unit, BM * BN, most);
+    return true;
+  }
+  __device__ __forceinline__ int work(const GemmArgs& g0) const {
+    GemmArgs g = g0;
+    Plan p;
+    return plan(g, p) ? p.s.full + p.s.rest * p.s.parts : 0;
+  }
+  __device__ __forceinline__ bool take(GemmArgs& g, int logical, int& ti, int& tj) {
+    Plan p;
+    plan(g, p);
+    int tile = logical;
+    if (logical >= p.s.full && p.s.parts > 1) {
+      slot = logical - p.s.full;
+      tile = p.s.full + slot / p.s.parts;
+      const int of = slot % p.s.parts, k0 = p.units * of / p.s.parts * kPadK;
+      g.K = p.units * (of + 1) / p.s.parts * kPadK - k0;
+      g.P = static_cast<const T*>(g.P) + (PT ? k0 * g.ldp : k0);
+      g.Q = static_cast<const T*>(g.Q) + (QN ? k0 * g.ldq : k0);
+    }
+    decode_tile<false>(tile, p.tm, p.tn, ti, tj);
+    row0 = ti * BM;
+    col0 = tj * BN;
+    return true;
+  }
+  __device__ __forceinline__ bool has_t() const { return false; }
+  __device__ __forceinline__ void load(int b, int i, int j0, int kbeg, int n, Pre& p, bool = false) const {
+    if (slot < 0) in.load(b, i, j0, kbeg, n, p);
+  }
+  __device__ __forceinline__ void load_t(int, int, int, int, PreT&, bool = false) const {}
+  __device__ __forceinline__ void put_t(int, int, int, const S*, int, const PreT&, bool = false) const {}
+  __device__ __forceinline__ void finish(int) const {}
+  __device__ __forceinline__ void put(int b, int i, int j0, const S* v, int kbeg, int n, const Pre& p, S* vo,
+                                      bool = false) const {
+    if (slot < 0)
+      in.put(b, i, j0, v, kbeg, n, p, vo);
+    else
+      st8<float, S>(part + ((int64_t)slot * BM + (i - row0)) * BN + (j0 - col0), v, kbeg, n);
+  }
+};
+
+// 16 rows of a tile in parts a workgroup.
+template <class Epi>
+__global__ void __launch_bounds__(256) join_parts_kernel(GemmArgs g, Epi epi) {
+  constexpr int BM = Epi::BM, BN = Epi::BN, RUNS = BN / 8;
+  typename Epi::Plan p;
+  if (!epi.plan(g, p) || p.s.parts == 1 || (int)blockIdx.x >= p.s.rest) return;
+  int ti, tj;
+  decode_tile<false>(p.s.full + blockIdx.x, p.tm, p.tn, ti, tj);
+  const float* part = epi.part + (int64_t)blockIdx.x * p.s.parts * BM * BN;
+#pragma unroll
+  for (int q = threadIdx.x; q < 16 * RUNS; q += 256) {
+    const int r = blockIdx.y * 16 + q / RUNS, c = q % RUNS * 8, i = ti * BM + r, j0 = tj * BN + c;
+    const int n = min(8, g.N - j0);
+    if (i >= g.M || n <= 0) continue;
+    typename Epi::Pre pre;
+    epi.in.load(0, i, j0, 0, n, pre);
+    float v[8] = {}, drop[8];
+#pragma unroll 4
+    for (int k = 0; k < p.s.parts; ++k) {
+      const float4* x = reinterpret_cast<const float4*>(part + ((int64_t)k * BM + r) * BN + c);
+      const float4 lo = x[0], hi = x[1];
+      v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
+      v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+    }
+    epi.in.put(0, i, j0, v, 0, n, pre, drop);
+  }
+}
+
+// x and y *= s[0] in place, nothing read where s[0] is 1 (the gradients of a
+// loss that is itself differentiated).
 template <typename T>
-__global__ void __launch_bounds__(256) scale_kernel(T* __restrict__ x, int64_t n, const float* __restrict__ s) {
+__global__ void __launch_bounds__(256) scale_kernel(T* __restrict__ x, int64_t n, T* __restrict__ y, int64_t m,
+                                                    const float* __restrict__ s) {
   const float f = s[0];
   if (f == 1.f) return;
   constexpr int E = 16 / (int)sizeof(T);
-  const int64_t step = (int64_t)gridDim.x * 256 * E;
-  for (int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * E; c < n; c += step) {
-    if (c + E <= n) {
-      uint4 u = ld16(x + c);
-      T* e = reinterpret_cast<T*>(&u);
+  const int64_t step = (int64_t)gridDim.x * 256 * E, first = ((int64_t)blockIdx.x * 256 + threadIdx.x) * E;
+  auto run = [&](T* p, int64_t len) {
+    for (int64_t c = first; c < len; c += step) {
+      if (c + E <= len) {
+        uint4 u = ld16(p + c);
+        T* e = reinterpret_cast<T*>(&u);
 #pragma unroll
-      for (int k = 0; k < E; ++k) e[k] = convert<T>(to_f(e[k]) * f);
-      st16(x + c, u);
-    } else {
-      for (int64_t k = c; k < n; ++k) x[k] = convert<T>(to_f(x[k]) * f);
+        for (int k = 0; k < E; ++k) e[k] = convert<T>(to_f(e[k]) * f);
+        st16(p + c, u);
+      } else {
+        for (int64_t k = c; k < len; ++k) p[k] = convert<T>(to_f(p[k]) * f);
+      }
     }
-  }
+  };
+  run(x, n);
+  run(y, m);
 }
 
 // ------------------------------------------------------------ host
@@ -1086,35 +1203,58 @@ struct Call {
 template <typename T>
 using Operand = std::conditional_t<sizeof(T) == 4, sp16, bf16>;
 
-// Parts of the vocabulary that dH of a chunk is split into: as many as leave
-// no CU idle through a long loop over K, each at least kPadK deep; the partial
-// sums (8 bytes of traffic an element) count against it. *tile: the faster
-// tile (pick_tile's 0 or 1).
-template <typename T>
-int grad_parts(int64_t rows, int64_t d, int64_t vp, int* tile) {
-  typedef TileSet<Operand<T>> Set;
-  typedef typename Set::big Big;
-  typedef typename Set::small Small;
-  const int64_t cus = device_cus(), units = vp / kPadK;
-  // microseconds of one unit of K on one CU, per element of a 256² tile
-  const double us = (sizeof(T) == 2 ? 3.6 : 8.25) / 65536;
-  double best = 0;
-  int parts = 1;
-  for (int big = 0; big < 2; ++big) {
-    const int64_t bm = big ? Big::BM : Small::BM, bn = big ? Big::BN : Small::BN;
-    const int64_t tiles = ((rows + bm - 1) / bm) * ((d + bn - 1) / bn);
-    for (int p = 1; p <= 64 && p <= units; p *= 2) {
-      const double unit = bm * bn * us * (big ? 1.0 : Set::kBigRate);
-      double t = double((tiles * p + cus - 1) / cus) * ((units + p - 1) / p) * unit;
-      if (p > 1) t += 5 + p * (double)rows * d * 8 / 4e6;
-      if ((!big && p == 1) || t < best) {
-        best = t;
-        parts = p;
-        *tile = big;
-      }
-    }
+// Microseconds of kPadK of K of a tile on one CU.
+template <typename T, class Cfg>
+constexpr float tile_unit() {
+  return (sizeof(T) == 4 ? 8.25f : 3.6f) / 65536 * Cfg::BM * Cfg::BN *
+         (Cfg::BM == 256 ? 1.f : (float)TileSet<Operand<T>>::kBigRate);
+}
+// From this many rounds of tiles on, the last one is not worth parts.
+constexpr int kWholeRounds = 12;
+constexpr int64_t kPartFloats = 2 * 65536;  // per CU: two rounds of partial 256² tiles
+
+template <typename T, class Cfg, class In, bool QN, bool PT>
+int launch_gradient(const ArgsOf<Operand<T>>& args, const In& in, float* part, hipStream_t s, const char* name) {
+  typedef Operand<T> O;
+  typedef EpiSplit<In, Cfg, QN, PT, O> Epi;
+  ArgsOf<O> g = args;
+  PTO_REQUIRE(g.K % ring_k<O>() == 0 && g.ldq < (int64_t(1) << 26) && g.ldp < (int64_t(1) << 26) && g.ldp % 8 == 0 &&
+                  g.ldq % 8 == 0 && (!QN || g.ldq >= g.N) && (!PT || g.ldp >= g.M) &&
+                  ((reinterpret_cast<uintptr_t>(g.P) | reinterpret_cast<uintptr_t>(g.Q)) & 15) == 0,
+              std::string(name) + ": operands not padded or not 16-byte aligned");
+  g.tiles_m = (g.M + Cfg::BM - 1) / Cfg::BM;
+  g.tiles_n = (g.N + Cfg::BN - 1) / Cfg::BN;
+  g.cus = device_cus();
+  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
+  if (tiles == 0) return 0;
+  Epi e{in, part, tile_unit<T, Cfg>(), tiles >= kWholeRounds * g.cus ? 1 : kMostParts, g.cus};
+  const int64_t grid = tiles + (e.most > 1 ? 2 * g.cus : 0);
+  PTO_REQUIRE(grid < (1ll << 31), std::string(name) + ": grid too large");
+  ProfScope ps(name, s);
+  hipLaunchKernelGGL((gemm_nt_kernel<O, Cfg, false, Epi, QN, PT, false, ArgsOf<O>>), dim3((unsigned)grid), dim3(Cfg::NT),
+                     0, s, g, e);
+  PTO_LAUNCHED(name);
+  if (e.most > 1) {
+    hipLaunchKernelGGL(join_parts_kernel<Epi>, dim3((unsigned)std::min<int64_t>(tiles, g.cus), Cfg::BM / 16), dim3(256),
+                       0, s, static_cast<const GemmArgs&>(g), e);
+    PTO_LAUNCHED("join_parts");
   }
-  return parts;
+  return 0;
+}
+// With the tile that ends sooner if every row counts.
+template <typename T, bool QN, bool PT, class In>
+int launch_gradient(const ArgsOf<Operand<T>>& g, const In& in, float* part, hipStream_t s, const char* name) {
+  typedef typename TileSet<Operand<T>>::big Big;
+  typedef typename TileSet<Operand<T>>::small Small;
+  const int cus = device_cus(), units = g.K / kPadK;
+  auto time = [&](int bm, int bn, float unit) {
+    const int tiles = ((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn);
+    const Parts p = split_parts(tiles, units, cus, unit, bm * bn, kMostParts);
+    return p.time + (float)(p.full / cus) * units * unit;
+  };
+  if (time(Big::BM, Big::BN, tile_unit<T, Big>()) <= time(Small::BM, Small::BN, tile_unit<T, Small>()))
+    return launch_gradient<T, Big, In, QN, PT>(g, in, part, s, name);
+  return launch_gradient<T, Small, In, QN, PT>(g, in, part, s, name);
 }
 
 template <typename T>
@@ -1122,7 +1262,6 @@ struct Ws {
   static constexpr bool f32 = sizeof(T) == 4;
   int64_t dp, vp, blocks, cap, capp;
   bool pad_w;
-  int parts, part_tile = 0, part_len;
   Targets t{};
   int *list, *count;
   T* hc;
@@ -1131,11 +1270,11 @@ struct Ws {
   float *sums, *losses, *z, *caught, *alpha;
   RowsOut rows;
   T* kept;  // the kept logits, bf16: then S
-  // fp32: planes of H and W (by rows) for the logits, of S/a, W (transposed,
-  // S's exponents taken out) and a·H (by columns) for the gradients
-  sp16 *hp, *wpl, *sp, *wt, *ah;
-  int *eh, *ew, *es, *ewt, *eah;  // es and eah: exponents of the columns' maxima
-  unsigned* wpart;
+  // fp32: planes of H and W (by rows) for the logits, of S/a, W (S's exponents
+  // taken out) and a·H (by columns) for the gradients
+  sp16 *hp, *wpl, *sp, *ws, *ah;
+  int *eh, *ew, *es, *ews, *eah;  // es, ews and eah: exponents of the columns' maxima
+  float* undo;  // 2^-es
   float *part, *acc;
   int64_t chunks(const Call& c) const { return c.rows ? (c.rows + cap - 1) / cap : 0; }
   Ws(Carver& cv, const Call& c) {
@@ -1178,9 +1317,9 @@ struct Ws {
     rows = RowsOut{grads && (f32 || c.grad_rows) ? cv.take<RowSlope>(capp) : nullptr,
                    grads && (f32 || c.grad_rows) ? cv.take<float>(capp) : nullptr, nullptr};
     kept = grads ? cv.take<T>(capp * vp) : nullptr;
-    hp = wpl = sp = wt = ah = nullptr;
-    eh = ew = es = ewt = eah = nullptr;
-    wpart = nullptr;
+    hp = wpl = sp = ws = ah = nullptr;
+    eh = ew = es = ews = eah = nullptr;
+    undo = nullptr;
     if (f32) {
       hp = cv.take<sp16>(2 * capp * dp);
       wpl = cv.take<sp16>(2 * c.vocab * dp);
@@ -1188,20 +1327,18 @@ struct Ws {
       ew = cv.take<int>(c.vocab);
     }
     if (f32 && grads) {
-      rows.maxima = cv.take<unsigned>(vp + dp);
-      es = cv.take<int>(vp + dp);
+      rows.maxima = cv.take<unsigned>(vp + 2 * dp);
+      es = cv.take<int>(vp + 2 * dp);
       eah = es + vp;
+      ews = eah + dp;
       sp = cv.take<sp16>(2 * capp * vp);
       if (c.dw) ah = cv.take<sp16>(2 * capp * dp);
       if (c.dh) {
-        wt = cv.take<sp16>(2 * c.d * vp);
-        ewt = cv.take<int>(round_up(c.d, 8));
-        wpart = cv.take<unsigned>(round_up(c.d, 8) * absmax_col_parts(c.vocab));
+        ws = cv.take<sp16>(2 * vp * dp);
+        undo = cv.take<float>(vp + dp);
       }
     }
-    parts = c.dh ? grad_parts<T>(cap, c.d, vp, &part_tile) : 1;
-    part_len = (int)((vp / kPadK + parts - 1) / parts * kPadK);
-    part = parts > 1 ? cv.take<float>(parts * cap * dp) : nullptr;
+    part = grads ? cv.take<float>(kPartFloats * device_cus()) : nullptr;
     acc = !f32 && c.dw && chunks(c) > 1 ? cv.take<float>(c.vocab * c.d) : nullptr;
   }
 };
@@ -1227,28 +1364,16 @@ int launch_logits(const ArgsOf<Operand<T>>& g, const Epi& e, hipStream_t s) {
 // dH and dW of a chunk from its S.
 int chunk_gradients(const Call& c, const Ws<bf16>& w, const Chunk& ch, const bf16* W, int64_t ldw, bool first, bool last,
                     hipStream_t s) {
-  bf16 *dh = static_cast<bf16*>(c.dh), *dw = static_cast<bf16*>(c.dw);
-  if (dh && ch.cap > 0) {
-    GemmArgs g{w.kept, w.vp, 0, W, ldw, 0, ch.cap, (int)c.d, (int)w.vp, 0, 0, nullptr};
-    if (w.parts > 1) {
-      g.K = w.part_len;
-      g.sP = w.part_len;
-      g.sQ = w.part_len * ldw;
-      const EpiPart e{{}, ch, w.part, w.dp, w.cap * w.dp, w.part_len, (int)w.vp};
-      if (launch_gemm_qn(g, e, w.parts, s, "loss_dhidden", w.part_tile)) return -1;
-      hipLaunchKernelGGL(join_parts_kernel<bf16>, dim3((unsigned)ch.cap), dim3(256), 0, s, ch, w.part, w.dp,
-                         w.cap * w.dp, w.parts, c.d, w.alpha, dh);
-      PTO_LAUNCHED("join_parts");
-    } else {
-      const EpiRows<bf16> e{{}, ch, dh, c.d, w.alpha};
-      if (launch_gemm_qn(g, e, 1, s, "loss_dhidden", w.part_tile)) return -1;
-    }
+  if (c.dh && ch.cap > 0) {
+    const GemmArgs g{w.kept, w.vp, 0, W, ldw, 0, ch.cap, (int)c.d, (int)w.vp, 0, 0, nullptr};
+    const EpiRows<bf16> e{{}, ch, static_cast<bf16*>(c.dh), c.d, w.alpha};
+    if (launch_gradient<bf16, true, false>(g, e, w.part, s, "loss_dhidden")) return -1;
   }
-  if (dw) {
+  if (c.dw) {
     const int k = (int)round_up(ch.cap, kPadK);
     const GemmArgs g{w.kept, w.vp, 0, w.hc, w.dp, 0, (int)c.vocab, (int)c.d, k, 0, 0, nullptr};
-    const EpiWeight<bf16> e{{}, ch, w.acc, dw, c.d, first, last, w.alpha};
-    if (launch_gemm_qn<EpiWeight<bf16>, true>(g, e, 1, s, "loss_dweight")) return -1;
+    const EpiWeight<bf16> e{{}, ch, w.acc, static_cast<bf16*>(c.dw), c.d, first, last, w.alpha};
+    if (launch_gradient<bf16, true, true>(g, e, w.part, s, "loss_dweight")) return -1;
   }
   return 0;
 }
@@ -1256,64 +1381,51 @@ int chunk_gradients(const Call& c, const Ws<bf16>& w, const Chunk& ch, const bf1
 int chunk_gradients(const Call& c, const Ws<float>& w, const Chunk& ch, const LossSpec& sp, const float* z, bool first,
                     bool last, hipStream_t s) {
   float *dh = static_cast<float*>(c.dh), *dw = static_cast<float*>(c.dw);
-  const int k = (int)round_up(ch.cap, kPadK);
-  if (ch.cap > 0) {
-    hipLaunchKernelGGL(column_max_kernel<true>, dim3((unsigned)((w.vp + 1023) / 1024), (unsigned)((ch.cap + 63) / 64)),
-                       dim3(256), 0, s, ch, w.kept, w.vp, (int)c.vocab, w.rows.slope, w.rows.a, w.rows.maxima);
+  const int k = (int)round_up(ch.cap, kPadK), cap = ch.cap, vocab = (int)c.vocab, d = (int)c.d;
+  unsigned* const max_h = w.rows.maxima + w.vp;
+  auto columns = [](int64_t n, int64_t rows) { return dim3((unsigned)((n + 1023) / 1024), (unsigned)((rows + 63) / 64)); };
+  auto exponents = [&](const unsigned* maxima, int64_t n, int* e, float* undo) {
+    hipLaunchKernelGGL(exponents_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, maxima, n, e, undo);
+    PTO_LAUNCHED("exponents");
+    return 0;
+  };
+  if (cap > 0) {
+    hipLaunchKernelGGL(column_max_kernel<true>, columns(w.vp, cap), dim3(256), 0, s, ch, w.kept, w.vp, cap, vocab,
+                       w.rows.slope, w.rows.a, w.rows.maxima);
     PTO_LAUNCHED("column_max");
     if (dw) {
-      hipLaunchKernelGGL(column_max_kernel<false>,
-                         dim3((unsigned)((w.dp + 1023) / 1024), (unsigned)((ch.cap + 63) / 64)), dim3(256), 0, s, ch,
-                         w.hc, w.dp, (int)c.d, w.rows.slope, w.rows.a, w.rows.maxima + w.vp);
+      hipLaunchKernelGGL(column_max_kernel<false>, columns(w.dp, cap), dim3(256), 0, s, ch, w.hc, w.dp, cap, d,
+                         w.rows.slope, w.rows.a, max_h);
       PTO_LAUNCHED("column_max");
     }
-    hipLaunchKernelGGL(exponents_kernel, dim3((unsigned)((w.vp + w.dp + 255) / 256)), dim3(256), 0, s, w.rows.maxima,
-                       w.vp + w.dp, w.es);
-    PTO_LAUNCHED("exponents");
-    hipLaunchKernelGGL(column_planes_kernel<true>, dim3((unsigned)k), dim3(256), 0, s, ch, w.kept, w.vp, (int)c.vocab,
-                       w.rows.slope, w.rows.a, w.es, w.sp, w.capp * w.vp, sp.k, w.t, z);
+    if (exponents(w.rows.maxima, w.vp + w.dp, w.es, w.undo)) return -1;
+    hipLaunchKernelGGL(column_planes_kernel<true>, dim3((unsigned)k), dim3(256), 0, s, ch, w.kept, w.vp, k, vocab,
+                       w.rows.slope, w.rows.a, w.es, w.sp, w.vp, w.capp * w.vp, sp.k, w.t, z);
     PTO_LAUNCHED("column_planes");
   }
-  if (dh && ch.cap > 0) {
-    SplitPack p{};
-    p.in = static_cast<const float*>(c.w);
-    p.rows = c.vocab;
-    p.cols = c.d;
-    p.ld_in = c.ldw;
-    p.cpart = w.wpart;
-    p.nw = round_up(c.d, 8);
-    p.ec = w.ewt;
-    p.out_t = w.wt;
-    p.pl_t = c.d * w.vp;
-    p.ld_t = w.vp;
-    p.pre_r = w.es;
-    p.pre_mul = -1;
-    p.pre_off = kSplitTop;
-    if (launch_split_pack_max(p, 1, s, false)) return -1;
-    SplitArgs g{{w.sp, w.vp, 0, w.wt, w.vp, 0, ch.cap, (int)c.d, (int)w.vp}, w.capp * w.vp, c.d * w.vp};
-    if (w.parts > 1) {
-      g.K = w.part_len;
-      g.sP = w.part_len;
-      g.sQ = w.part_len;
-      const EpiPowers<EpiPart> e{{{}, ch, w.part, w.dp, w.cap * w.dp, w.part_len, (int)w.vp}, nullptr, w.ewt, -kSplitTop};
-      if (launch_gemm<sp16, false>(g, e, w.parts, s, "loss_dhidden")) return -1;
-      hipLaunchKernelGGL(join_parts_kernel<float>, dim3((unsigned)ch.cap), dim3(256), 0, s, ch, w.part, w.dp,
-                         w.cap * w.dp, w.parts, c.d, w.rows.a, dh);
-      PTO_LAUNCHED("join_parts");
-    } else {
-      const EpiPowers<EpiRows<float>> e{{{}, ch, dh, c.d, w.rows.a}, nullptr, w.ewt, -kSplitTop};
-      if (launch_gemm<sp16, false>(g, e, 1, s, "loss_dhidden")) return -1;
-    }
+  if (dh && cap > 0) {
+    const Chunk all{nullptr, nullptr, 0, 0, vocab};
+    const float* W = static_cast<const float*>(c.w);
+    hipLaunchKernelGGL(column_max_kernel<false>, columns(w.dp, vocab), dim3(256), 0, s, all, W, c.ldw, vocab, d,
+                       w.rows.slope, w.undo, max_h + w.dp);
+    PTO_LAUNCHED("column_max");
+    if (exponents(max_h + w.dp, w.dp, w.ews, nullptr)) return -1;
+    hipLaunchKernelGGL(column_planes_kernel<false>, dim3((unsigned)w.vp), dim3(256), 0, s, all, W, c.ldw, (int)w.vp, d,
+                       w.rows.slope, w.undo, w.ews, w.ws, w.dp, w.vp * w.dp, sp.k, w.t, z);
+    PTO_LAUNCHED("column_planes");
+    const SplitArgs g{{w.sp, w.vp, 0, w.ws, w.dp, 0, cap, d, (int)w.vp}, w.capp * w.vp, w.vp * w.dp};
+    const EpiPowers<EpiRows<float>> e{{}, {{}, ch, dh, c.d, w.rows.a}, nullptr, w.ews, 0};
+    if (launch_gradient<float, true, false>(g, e, w.part, s, "loss_dhidden")) return -1;
   }
   if (dw) {
-    if (ch.cap > 0) {
-      hipLaunchKernelGGL(column_planes_kernel<false>, dim3((unsigned)k), dim3(256), 0, s, ch, w.hc, w.dp, (int)c.d,
-                         w.rows.slope, w.rows.a, w.eah, w.ah, w.capp * w.dp, sp.k, w.t, z);
+    if (cap > 0) {
+      hipLaunchKernelGGL(column_planes_kernel<false>, dim3((unsigned)k), dim3(256), 0, s, ch, w.hc, w.dp, k, d,
+                         w.rows.slope, w.rows.a, w.eah, w.ah, w.dp, w.capp * w.dp, sp.k, w.t, z);
       PTO_LAUNCHED("column_planes");
     }
-    const SplitArgs g{{w.sp, w.vp, 0, w.ah, w.dp, 0, (int)c.vocab, (int)c.d, k}, w.capp * w.vp, w.capp * w.dp};
-    const EpiPowers<EpiWeight<float>> e{{{}, ch, dw, dw, c.d, first, last, nullptr}, w.es, w.eah, 0};
-    if (launch_gemm_qn<EpiPowers<EpiWeight<float>>, true, false, sp16>(g, e, 1, s, "loss_dweight")) return -1;
+    const SplitArgs g{{w.sp, w.vp, 0, w.ah, w.dp, 0, vocab, d, k}, w.capp * w.vp, w.capp * w.dp};
+    const EpiPowers<EpiWeight<float>> e{{}, {{}, ch, dw, dw, c.d, first, last, nullptr}, w.es, w.eah, 0};
+    if (launch_gradient<float, true, true>(g, e, w.part, s, "loss_dweight")) return -1;
   }
   return 0;
 }
@@ -1364,7 +1476,7 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
       if constexpr (f32) {
         hipLaunchKernelGGL(gather_planes_kernel, dim3(capp / 4), dim3(256), 0, s, ch, static_cast<const float*>(c.h),
                            c.ldh, c.d, w.hc, w.dp, w.hp, w.capp * w.dp, w.eh, static_cast<float*>(c.dh), w.rows.maxima,
-                           grads ? w.vp + w.dp : 0);
+                           grads ? w.vp + 2 * w.dp : 0);
         g.P = w.hp;
         g.Q = w.wpl;
         g.ldq = w.dp;
@@ -1507,19 +1619,20 @@ int pto_linear_distillation(const void* hidden, int64_t ldh, const void* weight,
   return pto::run(c, dtype, workspace, ws_bytes, stream);
 }
 
-int pto_scale(void* x, int dtype, int64_t n, const float* factor, void* stream) {
-  PTO_REQUIRE(dtype == pto::kF32 || dtype == pto::kBF16, "scale: unsupported dtype code (fp32 and bf16)");
-  PTO_REQUIRE(n >= 0, "scale: negative extent");
-  PTO_REQUIRE(n == 0 || (x && factor), "scale: null operand");
-  if (n == 0) return 0;
+int pto_scale_pair(void* x, int64_t n, void* y, int64_t m, int dtype, const float* factor, void* stream) {
+  PTO_REQUIRE(dtype == pto::kF32 || dtype == pto::kBF16, "scale_pair: unsupported dtype code (fp32 and bf16)");
+  PTO_REQUIRE(n >= 0 && m >= 0, "scale_pair: negative extent");
+  PTO_REQUIRE((n == 0 || x) && (m == 0 || y) && (n + m == 0 || factor), "scale_pair: null operand");
+  if (n + m == 0) return 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned blocks = (unsigned)std::min<int64_t>((n + 2047) / 2048, 8 * pto::device_cus());
+  const unsigned blocks = (unsigned)std::min<int64_t>((std::max(n, m) + 2047) / 2048, 8 * pto::device_cus());
   if (dtype == pto::kBF16)
     hipLaunchKernelGGL(pto::scale_kernel<pto::bf16>, dim3(blocks), dim3(256), 0, s, static_cast<pto::bf16*>(x), n,
-                       factor);
+                       static_cast<pto::bf16*>(y), m, factor);
   else
-    hipLaunchKernelGGL(pto::scale_kernel<float>, dim3(blocks), dim3(256), 0, s, static_cast<float*>(x), n, factor);
-  PTO_LAUNCHED("scale");
+    hipLaunchKernelGGL(pto::scale_kernel<float>, dim3(blocks), dim3(256), 0, s, static_cast<float*>(x), n,
+                       static_cast<float*>(y), m, factor);
+  PTO_LAUNCHED("scale_pair");
   return 0;
 }
 

@@ -83,7 +83,7 @@ SIGNATURES = {
     "pto_linear_distillation": (_c_int, [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_int, _c_i64, _c_i64,
                                          _c_i64, _c_i64, _c_dbl, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                                          _c_ptr, _c_i64, _c_ptr, _c_size, _c_ptr]),
-    "pto_scale": (_c_int, [_c_ptr, _c_int, _c_i64, _c_ptr, _c_ptr]),
+    "pto_scale_pair": (_c_int, [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_int, _c_ptr, _c_ptr]),
     "pto_prof_enable": (_c_int, [_c_int]),
     "pto_prof_reset": (_c_int, []),
     "pto_prof_query": (_c_int, [ctypes.c_char_p, ctypes.POINTER(_c_dbl), ctypes.POINTER(_c_i64)]),

@@ -11,7 +11,8 @@ gradients under the rows' own.
 
 from __future__ import annotations
 
-import ctypes
+import contextlib
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -25,7 +26,12 @@ MAX_TEACHER = 1024
 
 
 def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
+
+
+def _on(device):
+    """The tensors' GPU as the current one; a switch costs more than the rest of a small call's host work."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _rows_readable(t):
@@ -33,27 +39,33 @@ def _rows_readable(t):
     return t if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(lib, *sizes):
+    return lib.pto_linear_loss_workspace_bytes(*sizes)
+
+
 class _Call:
     """One loss: its constants, and the C call that computes parts of it."""
 
-    def __init__(self, backend, what, labels, k, options, reduction):
+    def __init__(self, backend, what, dtype, labels, k, options, reduction):
         self.backend, self.what, self.labels, self.k = backend, what, labels, k
+        self.code = _DTYPE_CODE.get(dtype)
         self.options, self.reduction = options, _REDUCTION_CODE[reduction]
 
     def __call__(self, h, w, loss=None, norm=None, z=None, dh=None, dw=None, grad_rows=None):
         be, lib = self.backend, self.backend._lib
-        code, (rows, d), vocab = _DTYPE_CODE[h.dtype], h.shape, w.shape[0]
+        code, (rows, d), vocab = self.code, h.shape, w.shape[0]
         ldh = h.stride(0) if rows > 1 else d
         ldw = w.stride(0) if vocab > 1 else d
-        smoothing = self.options[1] if self.what == "linear_cross_entropy" else 0.0
-        with torch.cuda.device(h.device):
-            nbytes = lib.pto_linear_loss_workspace_bytes(code, rows, d, vocab, self.k, ldw, smoothing,
-                                                         int(self.what == "linear_distillation"), int(grad_rows is not None), int(dh is not None),
-                                                         int(dw is not None), be.LOSS_CHUNK_BYTES)
+        ce = self.what == "linear_cross_entropy"
+        sizes = (code, rows, d, vocab) if ce else (code, rows, d, vocab, self.k)
+        with _on(h.device):
+            nbytes = _workspace_bytes(lib, code, rows, d, vocab, self.k, ldw, self.options[1] if ce else 0.0, int(not ce),
+                                      int(grad_rows is not None), int(dh is not None), int(dw is not None),
+                                      be.LOSS_CHUNK_BYTES)
             ws = be._workspace(nbytes, h.device)
-            sizes = (code, rows, d, vocab) if self.what == "linear_cross_entropy" else (code, rows, d, vocab, self.k)
-            rc = getattr(lib, "pto_" + self.what)(
-                _ptr(h), ldh, _ptr(w), ldw, *(_ptr(t) for t in self.labels), *sizes, *self.options, self.reduction,
+            rc = (lib.pto_linear_cross_entropy if ce else lib.pto_linear_distillation)(
+                _ptr(h), ldh, _ptr(w), ldw, *map(_ptr, self.labels), *sizes, *self.options, self.reduction,
                 _ptr(grad_rows), _ptr(loss), _ptr(norm), _ptr(z), _ptr(dh), _ptr(dw), be.LOSS_CHUNK_BYTES, _ptr(ws),
                 nbytes, be._stream(h.device))
         be._check(rc, self.what)
@@ -104,16 +116,17 @@ class _LinearLoss(torch.autograd.Function):
         if grads is None:
             h, w = ctx.saved_tensors
             grads = call.gradients(h, w, ctx.needs, loss=torch.empty_like(grad))
-        for t in grads:
-            if t is not None:
-                with torch.cuda.device(t.device):
-                    rc = be._lib.pto_scale(_ptr(t), _DTYPE_CODE[t.dtype], t.numel(), _ptr(grad), be._stream(t.device))
-                be._check(rc, call.what)
-        return (*grads, None, None)
+        dh, dw = grads
+        with _on(grad.device):
+            rc = be._lib.pto_scale_pair(_ptr(dh), 0 if dh is None else dh.numel(), _ptr(dw),
+                                        0 if dw is None else dw.numel(), call.code, _ptr(grad),
+                                        be._stream(grad.device))
+        be._check(rc, call.what)
+        return dh, dw, None, None
 
 
 def _apply(call, hidden, weight, shape):
-    if hidden.dtype not in _DTYPE_CODE:
+    if call.code is None:
         raise OpsArgumentError(f"{call.what}: float32 and bfloat16 on the GPU, got {hidden.dtype}")
     on = torch.is_grad_enabled()
     needs = (on and hidden.requires_grad, on and weight.requires_grad)
@@ -132,7 +145,7 @@ def cross_entropy(backend, hidden, weight, targets, ignore_index, label_smoothin
     hidden, weight = _autocast(hidden, weight)
     reference.check_cross_entropy(hidden, weight, targets, label_smoothing, z_loss, reduction)
     labels = (targets.reshape(-1).to(torch.int64).contiguous(),)
-    call = _Call(backend, "linear_cross_entropy", labels, 1, (ignore_index, label_smoothing, z_loss), reduction)
+    call = _Call(backend, "linear_cross_entropy", hidden.dtype, labels, 1, (ignore_index, label_smoothing, z_loss), reduction)
     return _apply(call, hidden, weight, targets.shape)
 
 
@@ -144,5 +157,5 @@ def distillation(backend, hidden, weight, teacher_logits, teacher_index, tempera
         raise OpsArgumentError(f"linear_distillation: at most {MAX_TEACHER} teacher entries per row, got {k}")
     labels = (teacher_logits.detach().reshape(-1).to(torch.float32).contiguous(),
               teacher_index.reshape(-1).to(torch.int64).contiguous())
-    call = _Call(backend, "linear_distillation", labels, k, (temperature,), reduction)
+    call = _Call(backend, "linear_distillation", hidden.dtype, labels, k, (temperature,), reduction)
     return _apply(call, hidden, weight, teacher_index.shape[:-1])

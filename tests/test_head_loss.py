@@ -503,7 +503,8 @@ def test_library_refusals():
     rc = L.pto_linear_distillation(a, 8, a, 8, a, a, 0, 4, 8, 16, 4, 0.0, 1, None, a, None, None, None, None, 0, a,
                                    1 << 30, None)
     assert rc != 0 and b"temperature" in L.pto_last_error()
-    assert L.pto_scale(None, 0, 5, a, None) != 0 and L.pto_scale(None, 0, 0, None, None) == 0
+    assert L.pto_scale_pair(None, 5, None, 0, 0, a, None) != 0 and b"null" in L.pto_last_error()
+    assert L.pto_scale_pair(None, 0, None, 0, 0, None, None) == 0
     small = L.pto_linear_loss_workspace_bytes(2, 1, 2048, 32000, 1, 2048, 0.0, 0, 0, 0, 0, 0)
     assert 0 < small < 1 << 20  # scoring one token keeps no logits
     most = L.pto_linear_loss_workspace_bytes(2, 1 << 16, 4096, 128000, 1, 4096, 0.0, 0, 0, 1, 1, 0)
