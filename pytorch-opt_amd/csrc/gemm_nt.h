@@ -381,6 +381,8 @@ struct HasSkip<E, std::void_t<decltype(std::declval<const E&>().skip(0, false))>
 //       logical, int& ti, int& tj)`: the number of workgroups that have work (the
 //       launch has at least as many; the rest exit), and the tile of one of them,
 //       with g.P, g.Q and g.K moved to a part of K.
+//   `int p_row(int i) const`: the row of a K-contiguous P that output row i
+//       reads.
 //   `int q_rows() const`: rows of a K-contiguous Q that exist, where N
 //       counts the padded columns of the output (the rest re-read the last).
 template <class E, class = void>
@@ -393,6 +395,10 @@ struct HasWork : std::false_type {};
 template <class E>
 struct HasWork<E, std::void_t<decltype(std::declval<const E&>().work(std::declval<const GemmArgs&>()))>>
     : std::true_type {};
+template <class E, class = void>
+struct HasPRow : std::false_type {};
+template <class E>
+struct HasPRow<E, std::void_t<decltype(std::declval<const E&>().p_row(0))>> : std::true_type {};
 template <class E, class = void>
 struct HasQRows : std::false_type {};
 template <class E>
@@ -803,7 +809,8 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_nt_kernel(Args g, Epi epi) {
       s = static_cast<const T*>(g.P) + (int64_t)b * g.sP + (int64_t)rp * g.ldp + col;
       step[q] = (unsigned)(kRowBytes * g.ldp);
     } else if (R0 < BM) {
-      const int gr = min(row0 + r, max(g.M - 1, 0));
+      int gr = min(row0 + r, max(g.M - 1, 0));
+      if constexpr (HasPRow<Epi>::value) gr = epi.p_row(gr);
       s = static_cast<const T*>(g.P) + (int64_t)b * g.sP + (int64_t)gr * g.ldp + chunk * VEC;
       step[q] = kRowBytes;
     } else if (!QN) {

@@ -465,10 +465,12 @@ struct EpiLogits {
   Targets tg;
   int k;
   float* targets;  // [cap][k], null: the targets' logits t, by rank
+  bool in_place;   // P is H itself, its rows by the list
   __device__ __forceinline__ bool adjust(GemmArgs& g, int, int row0, int) const {
     g.M = SLOPE ? ch.padded() : ch.live();
     return row0 < g.M;
   }
+  __device__ __forceinline__ int p_row(int i) const { return in_place ? ch.list[ch.base + i] : i; }
   __device__ __forceinline__ int q_rows() const { return vocab; }
   __device__ __forceinline__ void finish(int) const {}
   template <class V, int FM, int FN>
@@ -841,7 +843,9 @@ __global__ void __launch_bounds__(64) put_targets_kernel(Chunk ch, int k, Target
 }
 
 // The loss of the call: a sum in a fixed order, over the count for the mean
-// (no row counts: 0).
+// (no row counts: 0). A launch of its own (4 us): a counter that lets the last
+// finish workgroup do it costs every one a release, which writes an XCD's L2
+// back (8192 rows of 32000: +450 us).
 __global__ void __launch_bounds__(1024) reduce_loss_kernel(const float* __restrict__ losses, int64_t rows,
                                                            const int* __restrict__ count, int mean,
                                                            float* __restrict__ out) {
@@ -855,7 +859,7 @@ __global__ void __launch_bounds__(1024) reduce_loss_kernel(const float* __restri
     if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
     __syncthreads();
   }
-  if (threadIdx.x == 0) out[0] = (float)(red[0] / (mean && rows ? max(1, count[0]) : 1));
+  if (threadIdx.x == 0) out[0] = (float)(red[0] / (mean ? max(1, count[0]) : 1));
 }
 
 // fp32: S/a and a·H as split planes for the gradients' products. dW sums over
@@ -1227,7 +1231,11 @@ int launch_gradient(const ArgsOf<Operand<T>>& args, const In& in, float* part, h
   g.cus = device_cus();
   const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
   if (tiles == 0) return 0;
-  Epi e{in, part, tile_unit<T, Cfg>(), tiles >= kWholeRounds * g.cus ? 1 : kMostParts, g.cus};
+  // dW's tiles are known here, and fewer rows make parts pay less
+  const bool whole = tiles >= kWholeRounds * g.cus ||
+                     (PT && split_parts((int)tiles, g.K / kPadK, g.cus, tile_unit<T, Cfg>(), Cfg::BM * Cfg::BN,
+                                        kMostParts).parts == 1);
+  Epi e{in, part, tile_unit<T, Cfg>(), whole ? 1 : kMostParts, g.cus};
   const int64_t grid = tiles + (e.most > 1 ? 2 * g.cus : 0);
   PTO_REQUIRE(grid < (1ll << 31), std::string(name) + ": grid too large");
   ProfScope ps(name, s);
@@ -1261,7 +1269,7 @@ template <typename T>
 struct Ws {
   static constexpr bool f32 = sizeof(T) == 4;
   int64_t dp, vp, blocks, cap, capp;
-  bool pad_w;
+  bool pad_w, in_place;
   Targets t{};
   int *list, *count;
   T* hc;
@@ -1306,7 +1314,9 @@ struct Ws {
     list = cv.take<int>(c.rows);
     count = cv.take<int>(4);
     alpha = cv.take<float>(4);
-    hc = cv.take<T>(capp * dp);
+    // scoring reads aligned rows of H where they lie
+    in_place = !f32 && !grads && c.h && c.d % kPadK == 0 && c.ldh % 8 == 0 && (reinterpret_cast<uintptr_t>(c.h) & 15) == 0;
+    hc = in_place ? nullptr : cv.take<T>(capp * dp);
     wp = pad_w ? cv.take<bf16>(vp * dp) : nullptr;
     losses = cv.take<float>(c.rows);
     norm = cv.take<float2>(c.rows);
@@ -1482,6 +1492,9 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
         g.ldq = w.dp;
         g.pP = w.capp * w.dp;
         g.pQ = c.vocab * w.dp;
+      } else if (w.in_place) {
+        g.P = c.h;
+        g.ldp = c.ldh;
       } else {
         hipLaunchKernelGGL(gather_kernel, dim3(capp / 4), dim3(256), 0, s, ch, static_cast<const bf16*>(c.h), c.ldh,
                            c.d, w.hc, w.dp, static_cast<bf16*>(c.dh));
@@ -1498,12 +1511,12 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
         PTO_LAUNCHED("row_slopes");
         if constexpr (f32) {
           const EpiLogits<T, true, false> e{ch,      (int)c.vocab, scale, w.stats, nullptr, w.blocks, w.kept,
-                                            w.vp,    nullptr,      w.eh,  w.ew,    w.t,     sp.k,     nullptr};
+                                            w.vp,    nullptr,      w.eh,  w.ew,    w.t,     sp.k,     nullptr, false};
           if (launch_logits<T>(g, e, s)) return -1;
         } else {
           g.M = (int)capp;
           const EpiLogits<T, false, true> e{ch,   (int)c.vocab, scale,   nullptr, nullptr, w.blocks, w.kept,
-                                            w.vp, w.rows.slope, nullptr, nullptr, w.t,     sp.k,     nullptr};
+                                            w.vp, w.rows.slope, nullptr, nullptr, w.t,     sp.k,     nullptr, false};
           if (launch_logits<T>(g, e, s)) return -1;
           hipLaunchKernelGGL(put_targets_kernel, dim3((unsigned)ch.cap), dim3(64), 0, s, ch, sp.k, w.t, z, w.rows,
                              w.kept, w.vp);
@@ -1513,7 +1526,7 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
         auto logits = [&](auto keep) {
           const EpiLogits<T, decltype(keep)::value, false> e{ch,     (int)c.vocab, scale, w.stats, w.sums,
                                                              w.blocks, w.kept,     w.vp,  nullptr, w.eh,
-                                                             w.ew,   w.t,          sp.k,  w.caught};
+                                                             w.ew,   w.t,          sp.k,  w.caught, w.in_place};
           return launch_logits<T>(g, e, s);
         };
         if (grads ? logits(std::true_type{}) : logits(std::false_type{})) return -1;

@@ -77,28 +77,33 @@ class _Call:
         return dh, dw
 
 
+def _readable(h, w):
+    h, w = _rows_readable(h), _rows_readable(w)
+    return h, w.clone(memory_format=torch.contiguous_format) if w.data_ptr() % 16 else w
+
+
+def _score(call, h, w):
+    h, w = _readable(h, w)
+    loss = torch.empty(() if call.reduction else h.shape[0], dtype=torch.float32, device=h.device)
+    call(h, w, loss=loss)
+    return loss
+
+
 class _LinearLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, w, call, needs):
         ctx.call, ctx.needs, ctx.grads = call, needs, None
-        h, w = _rows_readable(h), _rows_readable(w)
-        if w.data_ptr() % 16:
-            w = w.clone(memory_format=torch.contiguous_format)
+        h, w = _readable(h, w)
         if call.reduction:
             loss = torch.empty((), dtype=torch.float32, device=h.device)
-            if any(needs):
-                ctx.grads = call.gradients(h, w, needs, loss=loss)
-                ctx.save_for_backward(h, w)
-            else:
-                call(h, w, loss=loss)
+            ctx.grads = call.gradients(h, w, needs, loss=loss)
+            ctx.save_for_backward(h, w)
             return loss
         loss = torch.empty(h.shape[0], dtype=torch.float32, device=h.device)
-        norm = z = None
-        if any(needs):
-            norm = torch.empty(2 * h.shape[0], dtype=torch.float32, device=h.device)
-            z = torch.empty(h.shape[0] * call.k, dtype=torch.float32, device=h.device)
-            ctx.save_for_backward(h, w, norm, z)
+        norm = torch.empty(2 * h.shape[0], dtype=torch.float32, device=h.device)
+        z = torch.empty(h.shape[0] * call.k, dtype=torch.float32, device=h.device)
         call(h, w, loss=loss, norm=norm, z=z)
+        ctx.save_for_backward(h, w, norm, z)
         return loss
 
     @staticmethod
@@ -130,7 +135,8 @@ def _apply(call, hidden, weight, shape):
         raise OpsArgumentError(f"{call.what}: float32 and bfloat16 on the GPU, got {hidden.dtype}")
     on = torch.is_grad_enabled()
     needs = (on and hidden.requires_grad, on and weight.requires_grad)
-    loss = _LinearLoss.apply(hidden.reshape(-1, hidden.shape[-1]), weight, call, needs)
+    h = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
+    loss = _LinearLoss.apply(h, weight, call, needs) if any(needs) else _score(call, h.detach(), weight.detach())
     return loss if call.reduction else loss.reshape(shape)
 
 
