@@ -688,13 +688,6 @@ __device__ __forceinline__ RowSlope row_slope(const LossSpec& sp, float2 norm, f
 __device__ __forceinline__ float at_target(const RowSlope& rs, float a, float put, float z) {
   return fmaf(rs.pa, pow2(z - rs.m), fmaf(-a, put, rs.pu));
 }
-// S at a row's sparse targets, after the dense part was written.
-__device__ __forceinline__ void put_targets(bf16* srow, const RowSlope& rs, float a, const RowTargets& t,
-                                            const float* z, int first, int step) {
-  for (int e = first; e < t.k; e += step)
-    if (t.id(e) >= 0 && t.put(e) >= 0.f) srow[t.id(e)] = bf16(at_target(rs, a, t.put(e), z[e]));
-}
-
 // fp32: S/a of a row, its a, and the largest |S/a| of every column, as bits.
 struct RowsOut {
   RowSlope* slope;
@@ -715,7 +708,8 @@ struct RowsOut {
   }
 };
 
-// One workgroup per listed row: the normaliser, the loss and, for gradients
+// Workgroups (x) per listed row, each with a run of its columns (few rows would
+// leave CUs idle): the normaliser, the loss and, for gradients
 // (SLOPES), S/alpha in place of the kept logits (bf16) or what the passes over
 // them need (fp32). losses is per row of the call; norm (m, s) and z (the
 // targets' logits in the caller's order) per listed row.
@@ -726,10 +720,11 @@ __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __r
                                                      bf16* __restrict__ kept, int64_t ld, RowsOut out,
                                                      const float* __restrict__ alpha, float* __restrict__ losses,
                                                      float2* __restrict__ norms, float* __restrict__ z) {
-  const int i = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int i = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int64_t c0 = ld / kCols * blockIdx.x / gridDim.x * kCols, c1 = ld / kCols * (blockIdx.x + 1) / gridDim.x * kCols;
   if (i >= ch.live()) {
     if (SLOPES && sizeof(T) == 2 && i < ch.padded())
-      for (int64_t c = tid * 8; c < ld; c += 2048) *reinterpret_cast<uint4*>(kept + i * ld + c) = make_uint4(0, 0, 0, 0);
+      for (int64_t c = c0 + tid * 8; c < c1; c += 2048) *reinterpret_cast<uint4*>(kept + i * ld + c) = make_uint4(0, 0, 0, 0);
     return;
   }
   const int row = ch.list[ch.base + i];
@@ -758,7 +753,7 @@ __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __r
       ze = id < 0 ? NAN : caught[tg.one ? i : (int64_t)i * sp.k + tg.rank[(int64_t)i * sp.k + e]];
       qz += rt.q(e) * (ze - m);
     }
-    zr[e] = ze;
+    if (blockIdx.x == 0) zr[e] = ze;
   }
   s = wave_sum(s);
   sz = wave_sum(sz);
@@ -773,7 +768,7 @@ __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __r
   sz = red[2][0] + red[2][1] + red[2][2] + red[2][3];
   qz = red[3][0] + red[3][1] + red[3][2] + red[3][3];
   const float2 norm = make_float2(m, s);
-  if (tid == 0) {
+  if (tid == 0 && blockIdx.x == 0) {
     const double logs = log2((double)s);
     const double nat = kLn2 * (logs - ((double)qz + (double)sp.smooth * sz)) + rt.entropy();
     const double lse = kLn2 * ((double)m + logs);
@@ -786,7 +781,7 @@ __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __r
       return;
     }
     const RowSlope rs = row_slope(sp, norm, qz, 1.f);
-    for (int64_t c = tid * 8; c < ld; c += 2048) {
+    for (int64_t c = c0 + tid * 8; c < c1; c += 2048) {
       const uint4 u = *reinterpret_cast<const uint4*>(kept + i * ld + c);
       const unsigned uw[4] = {u.x, u.y, u.z, u.w};
       const float off = (st[c / kCols].x - m) - kOctaves;
@@ -800,7 +795,11 @@ __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __r
       st8<bf16, float>(kept + i * ld + c, o, 0, 8);
     }
     __syncthreads();  // the dense part is written before the targets' entries replace theirs
-    put_targets(kept + i * ld, rs, 1.f, rt, zr, tid, 256);
+    for (int e = tid; e < sp.k; e += 256) {
+      const int id = rt.id(e);
+      if (id >= c0 && id < c1 && rt.put(e) >= 0.f)
+        kept[i * ld + id] = bf16(at_target(rs, 1.f, rt.put(e), caught[tg.one ? i : (int64_t)i * sp.k + tg.rank[(int64_t)i * sp.k + e]]));
+    }
   }
 }
 
@@ -839,7 +838,9 @@ __global__ void __launch_bounds__(64) put_targets_kernel(Chunk ch, int k, Target
   const int i = blockIdx.x;
   if (i >= ch.live()) return;
   const int64_t at = ch.base + i;
-  put_targets(s + i * ld, rows.slope[i], rows.a[i], RowTargets{tg, at, ch.list[at], k}, z + at * k, threadIdx.x, 64);
+  const RowTargets t{tg, at, ch.list[at], k};
+  for (int e = threadIdx.x; e < k; e += 64)
+    if (t.id(e) >= 0 && t.put(e) >= 0.f) s[i * ld + t.id(e)] = bf16(at_target(rows.slope[i], rows.a[i], t.put(e), z[at * k + e]));
 }
 
 // The loss of the call: a sum in a fixed order, over the count for the mean
@@ -898,21 +899,23 @@ __global__ void __launch_bounds__(256) exponents_kernel(const unsigned* __restri
   e[c] = split_exp(__uint_as_float(maxima[c]));
   if (undo) undo[c] = ldexpf(1.f, -e[c]);
 }
-// The planes, one workgroup per row; pad rows and columns 0.
+// The planes, pad rows and columns 0: S/a by workgroups (x) with runs of a
+// row's columns, a·x by a wave per row.
 template <bool EXP>
 __global__ void __launch_bounds__(256) column_planes_kernel(Chunk ch, const float* __restrict__ x, int64_t ld, int rows,
                                                             int cols, const RowSlope* __restrict__ slope,
                                                             const float* __restrict__ a, const int* __restrict__ ec,
                                                             sp16* __restrict__ out, int64_t ldo, int64_t pl, int k,
-                                                            Targets tg,
-                                                            const float* __restrict__ z) {
-  const int i = blockIdx.x, tid = threadIdx.x;
+                                                            Targets tg, const float* __restrict__ z) {
+  const int tid = threadIdx.x, i = EXP ? blockIdx.y : blockIdx.x * 4 + (tid >> 6);
   if (i >= min(rows, ch.padded())) return;
+  const int64_t units = ldo / 8;
+  const int64_t c0 = EXP ? units * blockIdx.x / gridDim.x * 8 : 0, c1 = EXP ? units * (blockIdx.x + 1) / gridDim.x * 8 : ldo;
   const bool live = i < ch.live();
   sp16* o = out + i * ldo;
   const RowSlope rs = EXP && live ? slope[i] : RowSlope{0.f, 0.f, 0.f};
   const float ai = !EXP && live ? a[i] : 0.f;
-  for (int64_t c = tid * 8; c < ldo; c += 2048) {
+  for (int64_t c = c0 + (EXP ? tid : tid & 63) * 8; c < c1; c += EXP ? 2048 : 512) {
     float lo[4], hi[4], v[8];
     load_columns(x + i * ld + c, live ? cols - (int)c : 0, lo);
     load_columns(x + i * ld + c + 4, live ? cols - (int)c - 4 : 0, hi);
@@ -928,12 +931,12 @@ __global__ void __launch_bounds__(256) column_planes_kernel(Chunk ch, const floa
   }
   if constexpr (EXP) {
     if (!live) return;
-    __syncthreads();
+    __syncthreads();  // the dense part is written before the targets' entries replace theirs
     const int64_t at = ch.base + i;
     const RowTargets rt{tg, at, ch.list[at], k};
     for (int e = tid; e < k; e += 256) {
       const int id = rt.id(e);
-      if (id < 0 || !(rt.put(e) >= 0.f)) continue;
+      if (id < c0 || id >= c1 || !(rt.put(e) >= 0.f)) continue;
       const float w = ldexpf(at_target(rs, 1.f, rt.put(e), z[at * k + e]), ec[id]);
       const _Float16 h = static_cast<_Float16>(w);
       o[id].v = h;
@@ -1045,14 +1048,15 @@ struct Parts {
   int full, rest, parts;  // tiles in whole rounds, tiles left over, parts of each of those
   float time;
 };
-constexpr int kMostParts = 16;
+constexpr int kMostParts = 128;
 __host__ __device__ inline Parts split_parts(int tiles, int units, int cus, float unit, int area, int most) {
   Parts s;
   s.full = tiles / cus * cus;
   s.rest = tiles - s.full;
   s.parts = 1;
   s.time = s.rest > 0 ? units * unit : 0.f;
-  for (int p = 2; p <= most && p <= units && s.rest > 0 && s.rest * p <= 2 * cus; ++p) {
+  // 2, 3, 4, 6, 8, 12, ...
+  for (int p = 2; p <= most && p <= units && s.rest > 0 && s.rest * p <= 2 * cus; p += (p & (p - 1)) ? p / 3 : p / 2) {
     const float t = (float)((s.rest * p + cus - 1) / cus * ((units + p - 1) / p)) * unit + 7.f +
                     (float)s.rest * p * area * (8.f / 4.5e6f);
     if (t < s.time) {
@@ -1360,6 +1364,11 @@ size_t loss_ws_bytes(const Call& c) {
   return cv.used + 512;
 }
 
+// Workgroups per row of `cols`: two per CU in all, 2048 columns each at least.
+inline unsigned segments(int64_t rows, int64_t cols) {
+  return (unsigned)std::max<int64_t>(1, std::min<int64_t>(2 * device_cus() / rows, cols / 2048));
+}
+
 // The logits' product: 256² or 128² tiles, both of 64-column wave tiles.
 template <typename T, class Epi>
 int launch_logits(const ArgsOf<Operand<T>>& g, const Epi& e, hipStream_t s) {
@@ -1409,7 +1418,7 @@ int chunk_gradients(const Call& c, const Ws<float>& w, const Chunk& ch, const Lo
       PTO_LAUNCHED("column_max");
     }
     if (exponents(w.rows.maxima, w.vp + w.dp, w.es, w.undo)) return -1;
-    hipLaunchKernelGGL(column_planes_kernel<true>, dim3((unsigned)k), dim3(256), 0, s, ch, w.kept, w.vp, k, vocab,
+    hipLaunchKernelGGL(column_planes_kernel<true>, dim3(segments(k, w.vp), (unsigned)k), dim3(256), 0, s, ch, w.kept, w.vp, k, vocab,
                        w.rows.slope, w.rows.a, w.es, w.sp, w.vp, w.capp * w.vp, sp.k, w.t, z);
     PTO_LAUNCHED("column_planes");
   }
@@ -1420,7 +1429,7 @@ int chunk_gradients(const Call& c, const Ws<float>& w, const Chunk& ch, const Lo
                        w.rows.slope, w.undo, max_h + w.dp);
     PTO_LAUNCHED("column_max");
     if (exponents(max_h + w.dp, w.dp, w.ews, nullptr)) return -1;
-    hipLaunchKernelGGL(column_planes_kernel<false>, dim3((unsigned)w.vp), dim3(256), 0, s, all, W, c.ldw, (int)w.vp, d,
+    hipLaunchKernelGGL(column_planes_kernel<false>, dim3((unsigned)(w.vp / 4)), dim3(256), 0, s, all, W, c.ldw, (int)w.vp, d,
                        w.rows.slope, w.undo, w.ews, w.ws, w.dp, w.vp * w.dp, sp.k, w.t, z);
     PTO_LAUNCHED("column_planes");
     const SplitArgs g{{w.sp, w.vp, 0, w.ws, w.dp, 0, cap, d, (int)w.vp}, w.capp * w.vp, w.vp * w.dp};
@@ -1429,7 +1438,7 @@ int chunk_gradients(const Call& c, const Ws<float>& w, const Chunk& ch, const Lo
   }
   if (dw) {
     if (cap > 0) {
-      hipLaunchKernelGGL(column_planes_kernel<false>, dim3((unsigned)k), dim3(256), 0, s, ch, w.hc, w.dp, k, d,
+      hipLaunchKernelGGL(column_planes_kernel<false>, dim3((unsigned)(k / 4)), dim3(256), 0, s, ch, w.hc, w.dp, k, d,
                          w.rows.slope, w.rows.a, w.eah, w.ah, w.dp, w.capp * w.dp, sp.k, w.t, z);
       PTO_LAUNCHED("column_planes");
     }
@@ -1530,7 +1539,7 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
           return launch_logits<T>(g, e, s);
         };
         if (grads ? logits(std::true_type{}) : logits(std::false_type{})) return -1;
-        hipLaunchKernelGGL((grads ? finish_kernel<T, true> : finish_kernel<T, false>), dim3(capp), dim3(256), 0, s, ch,
+        hipLaunchKernelGGL((grads ? finish_kernel<T, true> : finish_kernel<T, false>), dim3(grads && !f32 ? segments(capp, w.vp) : 1, capp), dim3(256), 0, s, ch,
                            w.stats, w.sums, w.blocks, sp, w.t, w.caught, (int)c.vocab, reinterpret_cast<bf16*>(w.kept),
                            w.vp, w.rows, w.alpha, losses, norm, z);
         PTO_LAUNCHED("finish");
