@@ -383,6 +383,12 @@ struct HasSkip<E, std::void_t<decltype(std::declval<const E&>().skip(0, false))>
 //       with g.P, g.Q and g.K moved to a part of K.
 //   `int p_row(int i) const`: the row of a K-contiguous P that output row i
 //       reads.
+//   `const void* q_last() const`: where the last row of a K-contiguous Q lies
+//       whose rows are no whole rings of K tiles and run into the next (P holds
+//       zeros there); null: in its place.
+//   `int tail_tile() const` and `int64_t tail_bytes() const`: from this K tile
+//       on, a [K][N] Q lies so many bytes from where its rows would (a padded
+//       copy of its last ones).
 //   `int q_rows() const`: rows of a K-contiguous Q that exist, where N
 //       counts the padded columns of the output (the rest re-read the last).
 template <class E, class = void>
@@ -399,6 +405,14 @@ template <class E, class = void>
 struct HasPRow : std::false_type {};
 template <class E>
 struct HasPRow<E, std::void_t<decltype(std::declval<const E&>().p_row(0))>> : std::true_type {};
+template <class E, class = void>
+struct HasQLast : std::false_type {};
+template <class E>
+struct HasQLast<E, std::void_t<decltype(std::declval<const E&>().q_last())>> : std::true_type {};
+template <class E, class = void>
+struct HasTail : std::false_type {};
+template <class E>
+struct HasTail<E, std::enable_if_t<E::kTail>> : std::true_type {};
 template <class E, class = void>
 struct HasQRows : std::false_type {};
 template <class E>
@@ -818,6 +832,9 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_nt_kernel(Args g, Epi epi) {
       if constexpr (IsDirect<Epi>::value) qr = (qr & ~63) | ((qr & 15) << 2) | ((qr >> 4) & 3);
       const int gr = min(col0 + qr, max(qrows - 1, 0));
       s = static_cast<const T*>(g.Q) + (int64_t)b * g.sQ + (int64_t)gr * g.ldq + chunk * VEC;
+      if constexpr (HasQLast<Epi>::value) {
+        if (epi.q_last() && gr == qrows - 1) s = static_cast<const T*>(epi.q_last()) + chunk * VEC;
+      }
       step[q] = kRowBytes;
     } else {
       const int o = (R0 - BM) * kRowBytes + 16 * lane;
@@ -831,10 +848,20 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_nt_kernel(Args g, Epi epi) {
     if constexpr (kSplit) plane[q] = (R0 < BM ? g.pP : g.pQ) * (int64_t)sizeof(T);
     dst_off[q] = R0 * kRowBytes;
   }
+  int tail_tile = 0;
+  int64_t tail_bytes = 0;
+  if constexpr (HasTail<Epi>::value) {
+    tail_tile = epi.tail_tile();
+    tail_bytes = epi.tail_bytes();
+  }
   auto issue = [&](int kt, char* stage) {
 #pragma unroll
     for (int q = 0; q < IPW; ++q) {
       uint64_t off = (uint64_t)(unsigned)kt * step[q];
+      if constexpr (HasTail<Epi>::value) {
+        static_assert(QN && !kSplit, "a tail of a [K][N] operand");
+        if (16 * (wave * IPW + q) >= BM && kt >= tail_tile) off += tail_bytes;
+      }
       if constexpr (kSplit) off = (uint64_t)(unsigned)(kt >> 1) * step[q] + ((kt & 1) ? plane[q] : 0);
       __builtin_amdgcn_global_load_lds((gbl_void_t*)(src[q] + off), (lds_void_t*)(stage + dst_off[q]), 16, 0, 0);
     }

@@ -339,6 +339,17 @@ __global__ void __launch_bounds__(256) pad_weight_kernel(const bf16* __restrict_
   copy_row(w + min(r, vocab - 1) * ldw, r < vocab ? d : 0, out + r * ldo, ldo, threadIdx.x & 63);
 }
 
+// The rows of W from the last multiple of kPadK on, at W's pitch and with zero
+// rows up to the next (tail), and its last row by itself, padded to ldo.
+__global__ void __launch_bounds__(256) weight_tail_kernel(const bf16* __restrict__ w, int64_t ldw, int64_t vocab,
+                                                          int64_t d, bf16* __restrict__ tail, bf16* __restrict__ last,
+                                                          int64_t ldo) {
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int64_t v = vocab / kPadK * kPadK + r;
+  if (tail) copy_row(w + min(v, vocab - 1) * ldw, v < vocab ? d : 0, tail + r * ldw, ldw, lane);
+  if (last && r == 0) copy_row(w + (vocab - 1) * ldw, d, last, ldo, lane);
+}
+
 // Four values of a row of n (the rest 0).
 __device__ __forceinline__ void load_columns(const float* p, int n, float (&v)[4]) {
   uint4 u = make_uint4(0, 0, 0, 0);
@@ -466,11 +477,13 @@ struct EpiLogits {
   int k;
   float* targets;  // [cap][k], null: the targets' logits t, by rank
   bool in_place;   // P is H itself, its rows by the list
+  const void* last;  // a padded copy of W's last row, where its rows are read past their ends
   __device__ __forceinline__ bool adjust(GemmArgs& g, int, int row0, int) const {
     g.M = SLOPE ? ch.padded() : ch.live();
     return row0 < g.M;
   }
   __device__ __forceinline__ int p_row(int i) const { return in_place ? ch.list[ch.base + i] : i; }
+  __device__ __forceinline__ const void* q_last() const { return sizeof(T) == 2 ? last : nullptr; }
   __device__ __forceinline__ int q_rows() const { return vocab; }
   __device__ __forceinline__ void finish(int) const {}
   template <class V, int FM, int FN>
@@ -869,34 +882,60 @@ __global__ void __launch_bounds__(1024) reduce_loss_kernel(const float* __restri
 // the vocabulary, with the columns' exponents taken out of W's rows (undo); a,
 // which may differ by rows, multiplies its result.
 
-// Largest values of 1024 columns over 64 rows: of S/a (EXP, x = the logits) or
-// of a·x.
+// Largest values of columns over parts of the rows, parts[part][cols]: of S/a
+// (EXP, x = the logits) or of a·x. `across` threads (a power of two) take four
+// columns each, and the 256/across groups of them kPartRows rows each.
+constexpr int kPartRows = 64;
 template <bool EXP>
-__global__ void __launch_bounds__(256) column_max_kernel(Chunk ch, const float* __restrict__ x, int64_t ld, int rows, int cols,
-                                                         const RowSlope* __restrict__ slope,
-                                                         const float* __restrict__ a, unsigned* __restrict__ maxima) {
-  const int c = (blockIdx.x * 256 + threadIdx.x) * 4, r0 = blockIdx.y * 64, r1 = min(r0 + 64, min(rows, ch.live()));
-  if (c >= cols) return;
+__global__ void __launch_bounds__(256) column_max_kernel(Chunk ch, const float* __restrict__ x, int64_t ld, int rows,
+                                                         int cols, int across, const RowSlope* __restrict__ slope,
+                                                         const float* __restrict__ a, float* __restrict__ parts) {
+  __shared__ float part[256][4];
+  const int tid = threadIdx.x, groups = 256 / across, group = tid / across;
+  const int c = (blockIdx.x * across + tid % across) * 4;
+  const int r0 = (blockIdx.y * groups + group) * kPartRows, r1 = min(r0 + kPartRows, min(rows, ch.live()));
   float m[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < cols) {
 #pragma unroll 8
-  for (int i = r0; i < r1; ++i) {
-    float v[4];
-    load_columns(x + i * ld + c, cols - c, v);
+    for (int i = r0; i < r1; ++i) {
+      float v[4];
+      load_columns(x + i * ld + c, cols - c, v);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float w = fabsf(EXP ? fmaf(slope[i].pa, pow2(v[k] - slope[i].m), slope[i].pu) : a[i] * v[k]);
-      m[k] = w < INFINITY ? fmaxf(m[k], w) : m[k];
+      for (int k = 0; k < 4; ++k) {
+        const float w = fabsf(EXP ? fmaf(slope[i].pa, pow2(v[k] - slope[i].m), slope[i].pu) : a[i] * v[k]);
+        m[k] = w < INFINITY ? fmaxf(m[k], w) : m[k];
+      }
     }
   }
 #pragma unroll
+  for (int k = 0; k < 4; ++k) part[tid][k] = m[k];
+  __syncthreads();
+  if (group != 0 || c >= cols) return;
+  for (int g = 1; g < groups; ++g)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m[k] = fmaxf(m[k], part[g * across + tid][k]);
+#pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (c + k < cols && r0 < r1) atomicMax(&maxima[c + k], __float_as_uint(m[k]));
+    if (c + k < cols) parts[(int64_t)blockIdx.y * cols + c + k] = m[k];
 }
-__global__ void __launch_bounds__(256) exponents_kernel(const unsigned* __restrict__ maxima, int64_t n,
+// Exponents of n columns (pads to np: none) from the parts' maxima and, not
+// null, more of them; undo: 2^-e. 32 columns a workgroup.
+__global__ void __launch_bounds__(256) exponents_kernel(const float* __restrict__ parts, int count,
+                                                        const unsigned* __restrict__ more, int n, int np,
                                                         int* __restrict__ e, float* __restrict__ undo) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= n) return;
-  e[c] = split_exp(__uint_as_float(maxima[c]));
+  __shared__ float red[8][32];
+  const int g = threadIdx.x >> 5, c = blockIdx.x * 32 + (threadIdx.x & 31);
+  float m = 0.f;
+  if (c < n) {
+    if (more && g == 0) m = __uint_as_float(more[c]);
+#pragma unroll 8
+    for (int p = g; p < count; p += 8) m = fmaxf(m, parts[(int64_t)p * n + c]);
+  }
+  red[g][threadIdx.x & 31] = m;
+  __syncthreads();
+  if (g != 0 || c >= np) return;
+  for (int o = 1; o < 8; ++o) m = fmaxf(m, red[o][threadIdx.x]);
+  e[c] = split_exp(m);
   if (undo) undo[c] = ldexpf(1.f, -e[c]);
 }
 // The planes, pad rows and columns 0: S/a by workgroups (x) with runs of a
@@ -1069,7 +1108,7 @@ __host__ __device__ inline Parts split_parts(int tiles, int units, int cus, floa
 
 // Any of them, with the tiles of the last round in parts: partial tiles to the
 // workspace, joined by join_parts_kernel.
-template <class In, class Cfg, bool QN, bool PT, typename T>
+template <class In, class Cfg, bool QN, bool PT, typename T, bool TAIL>
 struct EpiSplit {
   typedef float S;
   typedef typename In::Pre Pre;
@@ -1080,7 +1119,12 @@ struct EpiSplit {
   float* part;
   float unit;
   int most, cus;
+  static constexpr bool kTail = TAIL;
+  int tail_k = 0;           // K from which Q's rows lie in a padded copy
+  int64_t tail_bytes_ = 0;  // and how far from their place
   int slot = -1, row0 = 0, col0 = 0;
+  __device__ __forceinline__ int tail_tile() const { return tail_k / Cfg::BK; }
+  __device__ __forceinline__ int64_t tail_bytes() const { return tail_bytes_; }
   struct Plan {
     Parts s;
     int tm, tn, units;
@@ -1109,6 +1153,7 @@ struct EpiSplit {
       g.K = p.units * (of + 1) / p.s.parts * kPadK - k0;
       g.P = static_cast<const T*>(g.P) + (PT ? k0 * g.ldp : k0);
       g.Q = static_cast<const T*>(g.Q) + (QN ? k0 * g.ldq : k0);
+      tail_k -= k0;
     }
     decode_tile<false>(tile, p.tm, p.tn, ti, tj);
     row0 = ti * BM;
@@ -1221,10 +1266,11 @@ constexpr float tile_unit() {
 constexpr int kWholeRounds = 12;
 constexpr int64_t kPartFloats = 2 * 65536;  // per CU: two rounds of partial 256² tiles
 
-template <typename T, class Cfg, class In, bool QN, bool PT>
-int launch_gradient(const ArgsOf<Operand<T>>& args, const In& in, float* part, hipStream_t s, const char* name) {
+template <typename T, class Cfg, class In, bool QN, bool PT, bool TAIL>
+int launch_gradient_cfg(const ArgsOf<Operand<T>>& args, const In& in, float* part, hipStream_t s, const char* name,
+                    int tail_k, const void* tail) {
   typedef Operand<T> O;
-  typedef EpiSplit<In, Cfg, QN, PT, O> Epi;
+  typedef EpiSplit<In, Cfg, QN, PT, O, TAIL> Epi;
   ArgsOf<O> g = args;
   PTO_REQUIRE(g.K % ring_k<O>() == 0 && g.ldq < (int64_t(1) << 26) && g.ldp < (int64_t(1) << 26) && g.ldp % 8 == 0 &&
                   g.ldq % 8 == 0 && (!QN || g.ldq >= g.N) && (!PT || g.ldp >= g.M) &&
@@ -1240,6 +1286,10 @@ int launch_gradient(const ArgsOf<Operand<T>>& args, const In& in, float* part, h
                      (PT && split_parts((int)tiles, g.K / kPadK, g.cus, tile_unit<T, Cfg>(), Cfg::BM * Cfg::BN,
                                         kMostParts).parts == 1);
   Epi e{in, part, tile_unit<T, Cfg>(), whole ? 1 : kMostParts, g.cus};
+  if (TAIL) {
+    e.tail_k = tail_k;
+    e.tail_bytes_ = static_cast<const char*>(tail) - static_cast<const char*>(g.Q) - (int64_t)tail_k * g.ldq * (int64_t)sizeof(O);
+  }
   const int64_t grid = tiles + (e.most > 1 ? 2 * g.cus : 0);
   PTO_REQUIRE(grid < (1ll << 31), std::string(name) + ": grid too large");
   ProfScope ps(name, s);
@@ -1255,7 +1305,8 @@ int launch_gradient(const ArgsOf<Operand<T>>& args, const In& in, float* part, h
 }
 // With the tile that ends sooner if every row counts.
 template <typename T, bool QN, bool PT, class In>
-int launch_gradient(const ArgsOf<Operand<T>>& g, const In& in, float* part, hipStream_t s, const char* name) {
+int launch_gradient(const ArgsOf<Operand<T>>& g, const In& in, float* part, hipStream_t s, const char* name,
+                    int tail_k = 0, const void* tail = nullptr) {
   typedef typename TileSet<Operand<T>>::big Big;
   typedef typename TileSet<Operand<T>>::small Small;
   const int cus = device_cus(), units = g.K / kPadK;
@@ -1264,9 +1315,28 @@ int launch_gradient(const ArgsOf<Operand<T>>& g, const In& in, float* part, hipS
     const Parts p = split_parts(tiles, units, cus, unit, bm * bn, kMostParts);
     return p.time + (float)(p.full / cus) * units * unit;
   };
-  if (time(Big::BM, Big::BN, tile_unit<T, Big>()) <= time(Small::BM, Small::BN, tile_unit<T, Small>()))
-    return launch_gradient<T, Big, In, QN, PT>(g, in, part, s, name);
-  return launch_gradient<T, Small, In, QN, PT>(g, in, part, s, name);
+  const bool big = time(Big::BM, Big::BN, tile_unit<T, Big>()) <= time(Small::BM, Small::BN, tile_unit<T, Small>());
+  if constexpr (QN && !PT && sizeof(T) == 2) {
+    if (tail)
+      return big ? launch_gradient_cfg<T, Big, In, QN, PT, true>(g, in, part, s, name, tail_k, tail)
+                 : launch_gradient_cfg<T, Small, In, QN, PT, true>(g, in, part, s, name, tail_k, tail);
+  }
+  return big ? launch_gradient_cfg<T, Big, In, QN, PT, false>(g, in, part, s, name, 0, nullptr)
+             : launch_gradient_cfg<T, Small, In, QN, PT, false>(g, in, part, s, name, 0, nullptr);
+}
+
+// Whether bf16 products read W where it lies, else from a padded copy. They can
+// where its rows are 16-byte aligned and what follows a row's end up to a
+// multiple of kPadK is nothing but the next row (an infinity there times H's
+// zero makes a NaN of a row that it would have made infinite itself), and do
+// where nothing needs padding or the rows of H are few. Copying costs a read and
+// a write of W, 5001 x 1000 x 50001 (2000 rows count) 32 us; reading in place
+// rows that are no whole 128-byte lines 50, a tail of the vocabulary 5% of dH
+// (8192 x 2048 x 32000: 15 against 53 for the copy, 64 x 2240 x 35072: 2
+// against 52).
+inline bool reads_in_place(const Call& c, int64_t dp) {
+  if (c.ldw % 8 || (c.d % kPadK && (c.ldw != c.d || dp - c.d > c.d))) return false;
+  return (c.d % kPadK == 0 && (!c.dh || c.vocab % kPadK == 0)) || c.rows <= (c.ldw % 64 ? 1024 : 8192);
 }
 
 template <typename T>
@@ -1277,7 +1347,9 @@ struct Ws {
   Targets t{};
   int *list, *count;
   T* hc;
-  bf16* wp;  // bf16: W padded
+  // bf16: W padded; or its last rows up to a multiple of kPadK and, by itself,
+  // its last one
+  bf16 *wp, *tail, *last;
   float2 *stats, *norm;
   float *sums, *losses, *z, *caught, *alpha;
   RowsOut rows;
@@ -1286,7 +1358,7 @@ struct Ws {
   // taken out) and a·H (by columns) for the gradients
   sp16 *hp, *wpl, *sp, *ws, *ah;
   int *eh, *ew, *es, *ews, *eah;  // es, ews and eah: exponents of the columns' maxima
-  float* undo;  // 2^-es
+  float *undo, *parts;  // 2^-es; maxima of parts of the rows
   float *part, *acc;
   int64_t chunks(const Call& c) const { return c.rows ? (c.rows + cap - 1) / cap : 0; }
   Ws(Carver& cv, const Call& c) {
@@ -1298,7 +1370,7 @@ struct Ws {
     cap = (c.chunk_bytes > 0 ? c.chunk_bytes : kChunkBytes) / per;
     cap = std::min(std::max<int64_t>(cap / 256 * 256, 256), std::max<int64_t>(c.rows, 1));
     capp = round_up(cap, kPadK);
-    pad_w = !f32 && (c.d % kPadK || c.ldw % 8 || (c.dh && c.vocab % kPadK));
+    pad_w = !f32 && !reads_in_place(c, dp);
     const bool join = !c.grad_rows;
     if (c.kd) {
       t.id = cv.take<int>(c.rows * c.k);
@@ -1322,6 +1394,8 @@ struct Ws {
     in_place = !f32 && !grads && c.h && c.d % kPadK == 0 && c.ldh % 8 == 0 && (reinterpret_cast<uintptr_t>(c.h) & 15) == 0;
     hc = in_place ? nullptr : cv.take<T>(capp * dp);
     wp = pad_w ? cv.take<bf16>(vp * dp) : nullptr;
+    tail = !f32 && !pad_w && c.dh && c.vocab % kPadK ? cv.take<bf16>(kPadK * c.ldw) : nullptr;
+    last = !f32 && !pad_w && c.d % kPadK ? cv.take<bf16>(dp) : nullptr;
     losses = cv.take<float>(c.rows);
     norm = cv.take<float2>(c.rows);
     z = cv.take<float>(c.rows * c.k);
@@ -1333,7 +1407,7 @@ struct Ws {
     kept = grads ? cv.take<T>(capp * vp) : nullptr;
     hp = wpl = sp = ws = ah = nullptr;
     eh = ew = es = ews = eah = nullptr;
-    undo = nullptr;
+    undo = parts = nullptr;
     if (f32) {
       hp = cv.take<sp16>(2 * capp * dp);
       wpl = cv.take<sp16>(2 * c.vocab * dp);
@@ -1341,15 +1415,16 @@ struct Ws {
       ew = cv.take<int>(c.vocab);
     }
     if (f32 && grads) {
-      rows.maxima = cv.take<unsigned>(vp + 2 * dp);
+      rows.maxima = cv.take<unsigned>(vp);
       es = cv.take<int>(vp + 2 * dp);
       eah = es + vp;
       ews = eah + dp;
+      parts = cv.take<float>(std::max((cap + kPartRows - 1) / kPartRows * vp, (c.vocab + kPartRows - 1) / kPartRows * dp));
       sp = cv.take<sp16>(2 * capp * vp);
       if (c.dw) ah = cv.take<sp16>(2 * capp * dp);
       if (c.dh) {
         ws = cv.take<sp16>(2 * vp * dp);
-        undo = cv.take<float>(vp + dp);
+        undo = cv.take<float>(vp);
       }
     }
     part = grads ? cv.take<float>(kPartFloats * device_cus()) : nullptr;
@@ -1386,7 +1461,8 @@ int chunk_gradients(const Call& c, const Ws<bf16>& w, const Chunk& ch, const bf1
   if (c.dh && ch.cap > 0) {
     const GemmArgs g{w.kept, w.vp, 0, W, ldw, 0, ch.cap, (int)c.d, (int)w.vp, 0, 0, nullptr};
     const EpiRows<bf16> e{{}, ch, static_cast<bf16*>(c.dh), c.d, w.alpha};
-    if (launch_gradient<bf16, true, false>(g, e, w.part, s, "loss_dhidden")) return -1;
+    if (launch_gradient<bf16, true, false>(g, e, w.part, s, "loss_dhidden", (int)(c.vocab / kPadK * kPadK), w.tail))
+      return -1;
   }
   if (c.dw) {
     const int k = (int)round_up(ch.cap, kPadK);
@@ -1401,23 +1477,24 @@ int chunk_gradients(const Call& c, const Ws<float>& w, const Chunk& ch, const Lo
                     bool last, hipStream_t s) {
   float *dh = static_cast<float*>(c.dh), *dw = static_cast<float*>(c.dw);
   const int k = (int)round_up(ch.cap, kPadK), cap = ch.cap, vocab = (int)c.vocab, d = (int)c.d;
-  unsigned* const max_h = w.rows.maxima + w.vp;
-  auto columns = [](int64_t n, int64_t rows) { return dim3((unsigned)((n + 1023) / 1024), (unsigned)((rows + 63) / 64)); };
-  auto exponents = [&](const unsigned* maxima, int64_t n, int* e, float* undo) {
-    hipLaunchKernelGGL(exponents_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, maxima, n, e, undo);
+  // the exponents of the columns (np with pads) of S/a or a·x
+  auto exponents = [&](auto exp, const Chunk& of, const float* x, int64_t ld, int rows, int cols, int64_t np,
+                       const float* a, int* e, float* undo) {
+    int across = 256;
+    while (across > 16 && across * 2 >= cols) across /= 2;
+    const int each = 256 / across * kPartRows, count = (rows + each - 1) / each;
+    hipLaunchKernelGGL((column_max_kernel<decltype(exp)::value>),
+                       dim3((unsigned)((cols + across * 4 - 1) / (across * 4)), (unsigned)count), dim3(256), 0, s, of, x,
+                       ld, rows, cols, across, w.rows.slope, a, w.parts);
+    PTO_LAUNCHED("column_max");
+    hipLaunchKernelGGL(exponents_kernel, dim3((unsigned)((np + 31) / 32)), dim3(256), 0, s, w.parts, count,
+                       decltype(exp)::value ? w.rows.maxima : nullptr, cols, (int)np, e, undo);
     PTO_LAUNCHED("exponents");
     return 0;
   };
   if (cap > 0) {
-    hipLaunchKernelGGL(column_max_kernel<true>, columns(w.vp, cap), dim3(256), 0, s, ch, w.kept, w.vp, cap, vocab,
-                       w.rows.slope, w.rows.a, w.rows.maxima);
-    PTO_LAUNCHED("column_max");
-    if (dw) {
-      hipLaunchKernelGGL(column_max_kernel<false>, columns(w.dp, cap), dim3(256), 0, s, ch, w.hc, w.dp, cap, d,
-                         w.rows.slope, w.rows.a, max_h);
-      PTO_LAUNCHED("column_max");
-    }
-    if (exponents(w.rows.maxima, w.vp + w.dp, w.es, w.undo)) return -1;
+    if (exponents(std::true_type{}, ch, w.kept, w.vp, cap, vocab, w.vp, w.rows.a, w.es, w.undo)) return -1;
+    if (dw && exponents(std::false_type{}, ch, w.hc, w.dp, cap, d, w.dp, w.rows.a, w.eah, nullptr)) return -1;
     hipLaunchKernelGGL(column_planes_kernel<true>, dim3(segments(k, w.vp), (unsigned)k), dim3(256), 0, s, ch, w.kept, w.vp, k, vocab,
                        w.rows.slope, w.rows.a, w.es, w.sp, w.vp, w.capp * w.vp, sp.k, w.t, z);
     PTO_LAUNCHED("column_planes");
@@ -1425,10 +1502,7 @@ int chunk_gradients(const Call& c, const Ws<float>& w, const Chunk& ch, const Lo
   if (dh && cap > 0) {
     const Chunk all{nullptr, nullptr, 0, 0, vocab};
     const float* W = static_cast<const float*>(c.w);
-    hipLaunchKernelGGL(column_max_kernel<false>, columns(w.dp, vocab), dim3(256), 0, s, all, W, c.ldw, vocab, d,
-                       w.rows.slope, w.undo, max_h + w.dp);
-    PTO_LAUNCHED("column_max");
-    if (exponents(max_h + w.dp, w.dp, w.ews, nullptr)) return -1;
+    if (exponents(std::false_type{}, all, W, c.ldw, vocab, d, w.dp, w.undo, w.ews, nullptr)) return -1;
     hipLaunchKernelGGL(column_planes_kernel<false>, dim3((unsigned)(w.vp / 4)), dim3(256), 0, s, all, W, c.ldw, (int)w.vp, d,
                        w.rows.slope, w.undo, w.ews, w.ws, w.dp, w.vp * w.dp, sp.k, w.t, z);
     PTO_LAUNCHED("column_planes");
@@ -1483,6 +1557,9 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
       PTO_LAUNCHED("pad_weight");
       W = w.wp;
       ldw = w.dp;
+    } else if (w.tail || w.last) {
+      hipLaunchKernelGGL(weight_tail_kernel, dim3(kPadK / 4), dim3(256), 0, s, W, ldw, c.vocab, c.d, w.tail, w.last, w.dp);
+      PTO_LAUNCHED("weight_tail");
     }
   }
   const int64_t chunks = std::max<int64_t>(w.chunks(c), c.dw ? 1 : 0);  // no rows: dW is still written
@@ -1495,7 +1572,7 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
       if constexpr (f32) {
         hipLaunchKernelGGL(gather_planes_kernel, dim3(capp / 4), dim3(256), 0, s, ch, static_cast<const float*>(c.h),
                            c.ldh, c.d, w.hc, w.dp, w.hp, w.capp * w.dp, w.eh, static_cast<float*>(c.dh), w.rows.maxima,
-                           grads ? w.vp + 2 * w.dp : 0);
+                           grads ? w.vp : 0);
         g.P = w.hp;
         g.Q = w.wpl;
         g.ldq = w.dp;
@@ -1520,12 +1597,14 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
         PTO_LAUNCHED("row_slopes");
         if constexpr (f32) {
           const EpiLogits<T, true, false> e{ch,      (int)c.vocab, scale, w.stats, nullptr, w.blocks, w.kept,
-                                            w.vp,    nullptr,      w.eh,  w.ew,    w.t,     sp.k,     nullptr, false};
+                                            w.vp,    nullptr,      w.eh,  w.ew,    w.t,     sp.k,     nullptr, false,
+                                            w.last};
           if (launch_logits<T>(g, e, s)) return -1;
         } else {
           g.M = (int)capp;
           const EpiLogits<T, false, true> e{ch,   (int)c.vocab, scale,   nullptr, nullptr, w.blocks, w.kept,
-                                            w.vp, w.rows.slope, nullptr, nullptr, w.t,     sp.k,     nullptr, false};
+                                            w.vp, w.rows.slope, nullptr, nullptr, w.t,     sp.k,     nullptr, false,
+                                            w.last};
           if (launch_logits<T>(g, e, s)) return -1;
           hipLaunchKernelGGL(put_targets_kernel, dim3((unsigned)ch.cap), dim3(64), 0, s, ch, sp.k, w.t, z, w.rows,
                              w.kept, w.vp);
@@ -1535,7 +1614,8 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
         auto logits = [&](auto keep) {
           const EpiLogits<T, decltype(keep)::value, false> e{ch,     (int)c.vocab, scale, w.stats, w.sums,
                                                              w.blocks, w.kept,     w.vp,  nullptr, w.eh,
-                                                             w.ew,   w.t,          sp.k,  w.caught, w.in_place};
+                                                             w.ew,   w.t,          sp.k,  w.caught, w.in_place,
+                                                             w.last};
           return launch_logits<T>(g, e, s);
         };
         if (grads ? logits(std::true_type{}) : logits(std::false_type{})) return -1;
