@@ -568,7 +568,10 @@ struct EpiLogits {
             t[k] = fmaf(p.pa, pow2(fmaf(value(fm, r, k), scale, -p.m)), p.pu);
             if (!whole) t[k] = c0 + k < vocab ? t[k] : 0.f;
           }
-          if (i < g.M) st4(static_cast<T*>(kept) + i * ld + c0, t);
+          if (i < g.M)
+            st4(reinterpret_cast<T*>(static_cast<char*>(kept) + ((int64_t)(wr0 + fm * 16 + r) * ld + wc0) * (int64_t)sizeof(T) +
+                                     (unsigned)(sub * ld + 4 * l) * (unsigned)sizeof(T)),
+                t);
         }
       return;
     }
@@ -577,7 +580,14 @@ struct EpiLogits {
     // they lie, so it serves every row whose own maximum is at most 2^kNear
     // below; then a maximum per row (8 lane exchanges for each, half the
     // epilogue's instructions) is not needed.
-    if (whole) {
+    if (whole && wr0 + R <= g.M) {
+      // uniform row addresses and a 32-bit offset per lane: 64-bit products per
+      // lane and row cost 2 us a tile
+      char* const krow = static_cast<char*>(kept) + ((int64_t)wr0 * ld + wc0) * (int64_t)sizeof(T);
+      const unsigned klane = (unsigned)(sub * ld + 4 * l) * (unsigned)sizeof(T);
+      char* const srow = reinterpret_cast<char*>(stats + (int64_t)wr0 * blocks + wc0 / kCols);
+      const unsigned slane = (unsigned)((sub + (l & 3)) * blocks) * 8u;
+      const bool mine = (l & 12) == 0;
       // the order of non-negative floats is that of their bits; what is not a
       // number is above them all
       int top = 0;
@@ -594,7 +604,6 @@ struct EpiLogits {
       if (ref < INFINITY) {
 #pragma unroll
         for (int fm = 0; fm < FM; ++fm) {
-          const int i0 = wr0 + fm * 16 + sub;
           float s[4], z[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -604,16 +613,15 @@ struct EpiLogits {
             s[r] = (pow2(fmaf(v[0], scale, -ref)) + pow2(fmaf(v[1], scale, -ref))) +
                    (pow2(fmaf(v[2], scale, -ref)) + pow2(fmaf(v[3], scale, -ref)));
             if (sums) z[r] = (v[0] + v[1]) + (v[2] + v[3]);
-            if (KEEP && i0 + r < g.M) keep(i0 + r, c0, v, ref);
+            if (KEEP) keep(krow + (int64_t)(fm * 16 + r) * ld * (int64_t)sizeof(T), klane, v, ref);
           }
           // lane l: the sum of row r = l & 3
           const float sum = sum_rows(s, l);
           least = fminf(least, sum);
-          const bool mine = (l & 12) == 0 && i0 + (l & 3) < g.M;
-          if (mine) stats[(i0 + (l & 3)) * blocks + wc0 / kCols] = make_float2(ref, sum);
+          if (mine) *reinterpret_cast<float2*>(srow + (int64_t)(fm * 16) * blocks * 8 + slane) = make_float2(ref, sum);
           if (sums) {
             const float zs = sum_rows(z, l) * scale;
-            if (mine) sums[(i0 + (l & 3)) * blocks + wc0 / kCols] = zs;
+            if (mine) sums[(int64_t)(wr0 + fm * 16 + sub + (l & 3)) * blocks + wc0 / kCols] = zs;
           }
         }
         if (!__any(!(least >= kNear))) return;
@@ -621,6 +629,7 @@ struct EpiLogits {
     }
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
+      if (wr0 + fm * 16 >= g.M) break;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = wr0 + fm * 16 + sub + r;
@@ -645,22 +654,21 @@ struct EpiLogits {
           z = sum16(z) * scale;
           if (live && l == 0) sums[i * blocks + wc0 / kCols] = z;
         }
-        if (KEEP && live) keep(i, c0, v, ref);
+        if (KEEP && live) keep(static_cast<char*>(kept) + ((int64_t)i * ld + c0) * (int64_t)sizeof(T), 0, v, ref);
       }
     }
   }
   // Four columns of a row, kept.
-  __device__ __forceinline__ void keep(int64_t i, int c0, const float (&v)[4], float ref) const {
+  __device__ __forceinline__ void keep(char* row, unsigned at, const float (&v)[4], float ref) const {
     if constexpr (sizeof(T) == 2) {
       // 1 + (t − ref)/128 of 65535, rounded, between 0 and 65535
       const float f = scale / kOctaves, o = fmaf(-ref, 1.f / kOctaves, 1.f);
       auto two = [&](float a, float b) {
         return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(fmaf(a, f, o), fmaf(b, f, o)));
       };
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(kept) + i * ld + c0) = make_uint2(two(v[0], v[1]), two(v[2], v[3]));
+      *reinterpret_cast<uint2*>(row + at) = make_uint2(two(v[0], v[1]), two(v[2], v[3]));
     } else {
-      const float t[4] = {v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale};
-      st4(static_cast<float*>(kept) + i * ld + c0, t);
+      *reinterpret_cast<float4*>(row + at) = make_float4(v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale);
     }
   }
   template <typename U>
@@ -721,7 +729,7 @@ struct RowsOut {
   }
 };
 
-// Workgroups (x) per listed row, each with a run of its columns (few rows would
+// Workgroups (y) per listed row, each with a run of its columns (few rows would
 // leave CUs idle): the normaliser, the loss and, for gradients
 // (SLOPES), S/alpha in place of the kept logits (bf16) or what the passes over
 // them need (fp32). losses is per row of the call; norm (m, s) and z (the
@@ -733,8 +741,8 @@ __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __r
                                                      bf16* __restrict__ kept, int64_t ld, RowsOut out,
                                                      const float* __restrict__ alpha, float* __restrict__ losses,
                                                      float2* __restrict__ norms, float* __restrict__ z) {
-  const int i = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int64_t c0 = ld / kCols * blockIdx.x / gridDim.x * kCols, c1 = ld / kCols * (blockIdx.x + 1) / gridDim.x * kCols;
+  const int i = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int64_t c0 = ld / kCols * blockIdx.y / gridDim.y * kCols, c1 = ld / kCols * (blockIdx.y + 1) / gridDim.y * kCols;
   if (i >= ch.live()) {
     if (SLOPES && sizeof(T) == 2 && i < ch.padded())
       for (int64_t c = c0 + tid * 8; c < c1; c += 2048) *reinterpret_cast<uint4*>(kept + i * ld + c) = make_uint4(0, 0, 0, 0);
@@ -766,7 +774,7 @@ __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __r
       ze = id < 0 ? NAN : caught[tg.one ? i : (int64_t)i * sp.k + tg.rank[(int64_t)i * sp.k + e]];
       qz += rt.q(e) * (ze - m);
     }
-    if (blockIdx.x == 0) zr[e] = ze;
+    if (blockIdx.y == 0) zr[e] = ze;
   }
   s = wave_sum(s);
   sz = wave_sum(sz);
@@ -781,7 +789,7 @@ __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __r
   sz = red[2][0] + red[2][1] + red[2][2] + red[2][3];
   qz = red[3][0] + red[3][1] + red[3][2] + red[3][3];
   const float2 norm = make_float2(m, s);
-  if (tid == 0 && blockIdx.x == 0) {
+  if (tid == 0 && blockIdx.y == 0) {
     const double logs = log2((double)s);
     const double nat = kLn2 * (logs - ((double)qz + (double)sp.smooth * sz)) + rt.entropy();
     const double lse = kLn2 * ((double)m + logs);
@@ -892,8 +900,8 @@ __global__ void __launch_bounds__(256) column_max_kernel(Chunk ch, const float* 
                                                          const float* __restrict__ a, float* __restrict__ parts) {
   __shared__ float part[256][4];
   const int tid = threadIdx.x, groups = 256 / across, group = tid / across;
-  const int c = (blockIdx.x * across + tid % across) * 4;
-  const int r0 = (blockIdx.y * groups + group) * kPartRows, r1 = min(r0 + kPartRows, min(rows, ch.live()));
+  const int c = (blockIdx.y * across + tid % across) * 4;
+  const int r0 = (blockIdx.x * groups + group) * kPartRows, r1 = min(r0 + kPartRows, min(rows, ch.live()));
   float m[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < cols) {
 #pragma unroll 8
@@ -916,7 +924,7 @@ __global__ void __launch_bounds__(256) column_max_kernel(Chunk ch, const float* 
     for (int k = 0; k < 4; ++k) m[k] = fmaxf(m[k], part[g * across + tid][k]);
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (c + k < cols) parts[(int64_t)blockIdx.y * cols + c + k] = m[k];
+    if (c + k < cols) parts[(int64_t)blockIdx.x * cols + c + k] = m[k];
 }
 // Exponents of n columns (pads to np: none) from the parts' maxima and, not
 // null, more of them; undo: 2^-e. 32 columns a workgroup.
@@ -938,7 +946,7 @@ __global__ void __launch_bounds__(256) exponents_kernel(const float* __restrict_
   e[c] = split_exp(m);
   if (undo) undo[c] = ldexpf(1.f, -e[c]);
 }
-// The planes, pad rows and columns 0: S/a by workgroups (x) with runs of a
+// The planes, pad rows and columns 0: S/a by workgroups (y) with runs of a
 // row's columns, a·x by a wave per row.
 template <bool EXP>
 __global__ void __launch_bounds__(256) column_planes_kernel(Chunk ch, const float* __restrict__ x, int64_t ld, int rows,
@@ -946,10 +954,10 @@ __global__ void __launch_bounds__(256) column_planes_kernel(Chunk ch, const floa
                                                             const float* __restrict__ a, const int* __restrict__ ec,
                                                             sp16* __restrict__ out, int64_t ldo, int64_t pl, int k,
                                                             Targets tg, const float* __restrict__ z) {
-  const int tid = threadIdx.x, i = EXP ? blockIdx.y : blockIdx.x * 4 + (tid >> 6);
+  const int tid = threadIdx.x, i = EXP ? blockIdx.x : blockIdx.x * 4 + (tid >> 6);
   if (i >= min(rows, ch.padded())) return;
   const int64_t units = ldo / 8;
-  const int64_t c0 = EXP ? units * blockIdx.x / gridDim.x * 8 : 0, c1 = EXP ? units * (blockIdx.x + 1) / gridDim.x * 8 : ldo;
+  const int64_t c0 = EXP ? units * blockIdx.y / gridDim.y * 8 : 0, c1 = EXP ? units * (blockIdx.y + 1) / gridDim.y * 8 : ldo;
   const bool live = i < ch.live();
   sp16* o = out + i * ldo;
   const RowSlope rs = EXP && live ? slope[i] : RowSlope{0.f, 0.f, 0.f};
@@ -1484,7 +1492,7 @@ int chunk_gradients(const Call& c, const Ws<float>& w, const Chunk& ch, const Lo
     while (across > 16 && across * 2 >= cols) across /= 2;
     const int each = 256 / across * kPartRows, count = (rows + each - 1) / each;
     hipLaunchKernelGGL((column_max_kernel<decltype(exp)::value>),
-                       dim3((unsigned)((cols + across * 4 - 1) / (across * 4)), (unsigned)count), dim3(256), 0, s, of, x,
+                       dim3((unsigned)count, (unsigned)((cols + across * 4 - 1) / (across * 4))), dim3(256), 0, s, of, x,
                        ld, rows, cols, across, w.rows.slope, a, w.parts);
     PTO_LAUNCHED("column_max");
     hipLaunchKernelGGL(exponents_kernel, dim3((unsigned)((np + 31) / 32)), dim3(256), 0, s, w.parts, count,
@@ -1495,7 +1503,7 @@ int chunk_gradients(const Call& c, const Ws<float>& w, const Chunk& ch, const Lo
   if (cap > 0) {
     if (exponents(std::true_type{}, ch, w.kept, w.vp, cap, vocab, w.vp, w.rows.a, w.es, w.undo)) return -1;
     if (dw && exponents(std::false_type{}, ch, w.hc, w.dp, cap, d, w.dp, w.rows.a, w.eah, nullptr)) return -1;
-    hipLaunchKernelGGL(column_planes_kernel<true>, dim3(segments(k, w.vp), (unsigned)k), dim3(256), 0, s, ch, w.kept, w.vp, k, vocab,
+    hipLaunchKernelGGL(column_planes_kernel<true>, dim3((unsigned)k, segments(k, w.vp)), dim3(256), 0, s, ch, w.kept, w.vp, k, vocab,
                        w.rows.slope, w.rows.a, w.es, w.sp, w.vp, w.capp * w.vp, sp.k, w.t, z);
     PTO_LAUNCHED("column_planes");
   }
@@ -1619,7 +1627,7 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
           return launch_logits<T>(g, e, s);
         };
         if (grads ? logits(std::true_type{}) : logits(std::false_type{})) return -1;
-        hipLaunchKernelGGL((grads ? finish_kernel<T, true> : finish_kernel<T, false>), dim3(grads && !f32 ? segments(capp, w.vp) : 1, capp), dim3(256), 0, s, ch,
+        hipLaunchKernelGGL((grads ? finish_kernel<T, true> : finish_kernel<T, false>), dim3(capp, grads && !f32 ? segments(capp, w.vp) : 1), dim3(256), 0, s, ch,
                            w.stats, w.sums, w.blocks, sp, w.t, w.caught, (int)c.vocab, reinterpret_cast<bf16*>(w.kept),
                            w.vp, w.rows, w.alpha, losses, norm, z);
         PTO_LAUNCHED("finish");

@@ -236,6 +236,41 @@ def test_chunks_of_rows(native_backend, dtype, keep, monkeypatch):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_rows_than_a_grid_is_high(native_backend, dtype):
+    """70001 rows in one chunk, a small vocabulary."""
+    h, w, g = _make(70001, 64, 40, dtype)
+    y = _targets(70001, 40, g, 0.99)
+    h.requires_grad_(), w.requires_grad_()
+    loss = ops.linear_cross_entropy(h, w, y, reduction="sum")
+    dh, dw = torch.autograd.grad(loss, (h, w))
+    _check(_exact_ce(h.detach(), w.detach(), y, reduction="sum"), loss.detach(), dh, dw, dtype, "sum")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [8, 40, 64, 72, 120, 192])
+def test_weights_read_past_their_rows(native_backend, dtype, d):
+    """Widths that need padding, the weight at the end of its allocation and
+    in the middle of one whose neighbours are not numbers."""
+    h, w, g = _make(50, d, 131, dtype)
+    y = _targets(50, 131, g)
+    pool = torch.full((3 * w.numel(),), float("nan"), dtype=dtype, device=DEV)
+    inner = pool[w.numel():2 * w.numel()].view_as(w).copy_(w)
+    wide = torch.full((131, d + 8), float("nan"), dtype=dtype, device=DEV)
+    slim = wide[:, :d].copy_(w)
+    want = None
+    for v in (w, inner, slim):
+        a, b = h.clone().requires_grad_(), v.detach().requires_grad_()
+        loss = ops.linear_cross_entropy(a, b, y)
+        got = (loss.detach(), *torch.autograd.grad(loss, (a, b)))
+        assert all(torch.isfinite(t).all() for t in got)
+        want = want or got
+        for s, t in zip(got, want):
+            assert torch.equal(s, t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strides_and_alignment(native_backend, dtype):
     """Views: a slice of wider rows, a weight off its alignment, transposed
     storage, leading dimensions, one shared row; the same values give the same
