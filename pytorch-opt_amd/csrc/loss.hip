@@ -912,17 +912,28 @@ __global__ void __launch_bounds__(256) column_max_kernel(Chunk ch, const float* 
   const int c = (blockIdx.y * across + tid % across) * 4;
   const int r0 = (blockIdx.x * groups + group) * kPartRows, r1 = min(r0 + kPartRows, min(rows, ch.live()));
   float m[4] = {0.f, 0.f, 0.f, 0.f};
-  if (c < cols) {
-#pragma unroll 8
-    for (int i = r0; i < r1; ++i) {
-      float v[4];
-      load_columns(x + i * ld + c, cols - c, v);
+  auto take = [&](int i, const float (&v)[4]) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float w = fabsf(EXP ? fmaf(slope[i].pa, pow2(v[k] - slope[i].m), slope[i].pu) : a[i] * v[k]);
-        m[k] = w < INFINITY ? fmaxf(m[k], w) : m[k];
-      }
+    for (int k = 0; k < 4; ++k) {
+      const float w = fabsf(EXP ? fmaf(slope[i].pa, pow2(v[k] - slope[i].m), slope[i].pu) : a[i] * v[k]);
+      m[k] = w < INFINITY ? fmaxf(m[k], w) : m[k];
     }
+  };
+  // eight rows' loads in flight
+  int i = c < cols ? r0 : r1;
+  if (cols - c >= 4)
+    for (; i + 8 <= r1; i += 8) {
+      uint4 u[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) u[q] = ld16(x + (i + q) * ld + c);
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        take(i + q, {__uint_as_float(u[q].x), __uint_as_float(u[q].y), __uint_as_float(u[q].z), __uint_as_float(u[q].w)});
+    }
+  for (; i < r1; ++i) {
+    float v[4];
+    load_columns(x + i * ld + c, cols - c, v);
+    take(i, v);
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) part[tid][k] = m[k];
@@ -971,19 +982,49 @@ __global__ void __launch_bounds__(256) column_planes_kernel(Chunk ch, const floa
   sp16* o = out + i * ldo;
   const RowSlope rs = EXP && live ? slope[i] : RowSlope{0.f, 0.f, 0.f};
   const float ai = !EXP && live ? a[i] : 0.f;
-  for (int64_t c = c0 + (EXP ? tid : tid & 63) * 8; c < c1; c += EXP ? 2048 : 512) {
-    float lo[4], hi[4], v[8];
-    load_columns(x + i * ld + c, live ? cols - (int)c : 0, lo);
-    load_columns(x + i * ld + c + 4, live ? cols - (int)c - 4 : 0, hi);
+  constexpr int STEP = EXP ? 2048 : 512;
+  auto put = [&](int64_t c, const uint4& lo, const uint4& hi, const int4& e0, const int4& e1) {
+    const unsigned u[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    const int e[8] = {e0.x, e0.y, e0.z, e0.w, e1.x, e1.y, e1.z, e1.w};
+    float v[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float y = k < 4 ? lo[k & 3] : hi[k & 3];
-      const float w = EXP ? fmaf(rs.pa, pow2(y - rs.m), rs.pu) : ai * y;
-      v[k] = live && c + k < cols ? ldexpf(w, ec[c + k]) : 0.f;
+      const float y = __uint_as_float(u[k]), w = EXP ? fmaf(rs.pa, pow2(y - rs.m), rs.pu) : ai * y;
+      v[k] = c + k < cols ? ldexpf(w, e[k]) : 0.f;
     }
     const Split8 s = split8(v);
     *reinterpret_cast<uint4*>(o + c) = s.h;
     *reinterpret_cast<uint4*>(o + pl + c) = s.l;
+  };
+  int64_t c = c0 + (EXP ? tid : tid & 63) * 8;
+  if (live) {
+    const float* xr = x + i * ld;
+    // two runs' loads in flight
+    for (; c + STEP + 8 <= min(c1, (int64_t)cols); c += 2 * STEP) {
+      uint4 u[4];
+      int4 e[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t at = c + (q >> 1) * STEP + (q & 1) * 4;
+        u[q] = ld16(xr + at);
+        e[q] = *reinterpret_cast<const int4*>(ec + at);
+      }
+      put(c, u[0], u[1], e[0], e[1]);
+      put(c + STEP, u[2], u[3], e[2], e[3]);
+    }
+    for (; c < min(c1, (int64_t)cols); c += STEP) {
+      float lo[4], hi[4];
+      load_columns(xr + c, cols - (int)c, lo);
+      load_columns(xr + c + 4, cols - (int)c - 4, hi);
+      uint4 u[2];
+      __builtin_memcpy(&u[0], lo, 16);
+      __builtin_memcpy(&u[1], hi, 16);
+      put(c, u[0], u[1], *reinterpret_cast<const int4*>(ec + c), *reinterpret_cast<const int4*>(ec + c + 4));
+    }
+  }
+  for (; c < c1; c += STEP) {
+    *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(o + pl + c) = make_uint4(0, 0, 0, 0);
   }
   if constexpr (EXP) {
     if (!live) return;
