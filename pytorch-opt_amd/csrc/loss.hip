@@ -1146,15 +1146,18 @@ struct Parts {
   float time;
 };
 constexpr int kMostParts = 128;
-__host__ __device__ inline Parts split_parts(int tiles, int units, int cus, float unit, int area, int most) {
+struct TileTime {
+  float unit, fixed;
+};
+__host__ __device__ inline Parts split_parts(int tiles, int units, int cus, TileTime tt, int area, int most) {
   Parts s;
   s.full = tiles / cus * cus;
   s.rest = tiles - s.full;
   s.parts = 1;
-  s.time = s.rest > 0 ? units * unit : 0.f;
+  s.time = s.rest > 0 ? units * tt.unit + tt.fixed : 0.f;
   // 2, 3, 4, 6, 8, 12, ...
   for (int p = 2; p <= most && p <= units && s.rest > 0 && s.rest * p <= 2 * cus; p += (p & (p - 1)) ? p / 3 : p / 2) {
-    const float t = (float)((s.rest * p + cus - 1) / cus * ((units + p - 1) / p)) * unit + 7.f +
+    const float t = (float)((s.rest * p + cus - 1) / cus) * ((units + p - 1) / p * tt.unit + tt.fixed) + 7.f +
                     (float)s.rest * p * area * (8.f / 4.5e6f);
     if (t < s.time) {
       s.time = t;
@@ -1175,7 +1178,7 @@ struct EpiSplit {
   static constexpr int BM = Cfg::BM, BN = Cfg::BN;
   In in;
   float* part;
-  float unit;
+  TileTime tt;
   int most, cus;
   static constexpr bool kTail = TAIL;
   int tail_k = 0;           // K from which Q's rows lie in a padded copy
@@ -1192,7 +1195,7 @@ struct EpiSplit {
     p.tm = (g.M + BM - 1) / BM;
     p.tn = (g.N + BN - 1) / BN;
     p.units = g.K / kPadK;
-    p.s = split_parts(p.tm * p.tn, p.units, cus, unit, BM * BN, most);
+    p.s = split_parts(p.tm * p.tn, p.units, cus, tt, BM * BN, most);
     return true;
   }
   __device__ __forceinline__ int work(const GemmArgs& g0) const {
@@ -1314,11 +1317,12 @@ struct Call {
 template <typename T>
 using Operand = std::conditional_t<sizeof(T) == 4, sp16, bf16>;
 
-// Microseconds of kPadK of K of a tile on one CU.
+// Microseconds of a tile on one CU (128² tiles run in twos), measured.
 template <typename T, class Cfg>
-constexpr float tile_unit() {
-  return (sizeof(T) == 4 ? 8.25f : 3.6f) / 65536 * Cfg::BM * Cfg::BN *
-         (Cfg::BM == 256 ? 1.f : (float)TileSet<Operand<T>>::kBigRate);
+constexpr TileTime tile_time() {
+  constexpr bool big = Cfg::BM == 256;
+  return {(sizeof(T) == 4 ? 8.25f : 3.6f) / 65536 * Cfg::BM * Cfg::BN * (big ? 1.f : (float)TileSet<Operand<T>>::kBigRate),
+          sizeof(T) == 4 ? (big ? 20.f : 5.f) : (big ? 11.5f : 3.5f)};
 }
 // From this many rounds of tiles on, the last one is not worth parts.
 constexpr int kWholeRounds = 12;
@@ -1341,9 +1345,9 @@ int launch_gradient_cfg(const ArgsOf<Operand<T>>& args, const In& in, float* par
   if (tiles == 0) return 0;
   // dW's tiles are known here, and fewer rows make parts pay less
   const bool whole = tiles >= kWholeRounds * g.cus ||
-                     (PT && split_parts((int)tiles, g.K / kPadK, g.cus, tile_unit<T, Cfg>(), Cfg::BM * Cfg::BN,
+                     (PT && split_parts((int)tiles, g.K / kPadK, g.cus, tile_time<T, Cfg>(), Cfg::BM * Cfg::BN,
                                         kMostParts).parts == 1);
-  Epi e{in, part, tile_unit<T, Cfg>(), whole ? 1 : kMostParts, g.cus};
+  Epi e{in, part, tile_time<T, Cfg>(), whole ? 1 : kMostParts, g.cus};
   if (TAIL) {
     e.tail_k = tail_k;
     e.tail_bytes_ = static_cast<const char*>(tail) - static_cast<const char*>(g.Q) - (int64_t)tail_k * g.ldq * (int64_t)sizeof(O);
@@ -1368,12 +1372,12 @@ int launch_gradient(const ArgsOf<Operand<T>>& g, const In& in, float* part, hipS
   typedef typename TileSet<Operand<T>>::big Big;
   typedef typename TileSet<Operand<T>>::small Small;
   const int cus = device_cus(), units = g.K / kPadK;
-  auto time = [&](int bm, int bn, float unit) {
+  auto time = [&](int bm, int bn, TileTime tt) {
     const int tiles = ((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn);
-    const Parts p = split_parts(tiles, units, cus, unit, bm * bn, kMostParts);
-    return p.time + (float)(p.full / cus) * units * unit;
+    const Parts p = split_parts(tiles, units, cus, tt, bm * bn, kMostParts);
+    return p.time + (float)(p.full / cus) * (units * tt.unit + tt.fixed);
   };
-  const bool big = time(Big::BM, Big::BN, tile_unit<T, Big>()) <= time(Small::BM, Small::BN, tile_unit<T, Small>());
+  const bool big = time(Big::BM, Big::BN, tile_time<T, Big>()) <= time(Small::BM, Small::BN, tile_time<T, Small>());
   if constexpr (QN && !PT && sizeof(T) == 2) {
     if (tail)
       return big ? launch_gradient_cfg<T, Big, In, QN, PT, true>(g, in, part, s, name, tail_k, tail)
@@ -1506,11 +1510,15 @@ inline unsigned segments(int64_t rows, int64_t cols) {
 template <typename T, class Epi>
 int launch_logits(const ArgsOf<Operand<T>>& g, const Epi& e, hipStream_t s) {
   typedef Operand<T> O;
+  typedef typename TileSet<O>::big Big;
+  typedef Tile<128, 128, 32, 2, 2> Small;
   const int64_t cus = device_cus();
-  auto rounds = [&](int64_t b) { return double(((g.M + b - 1) / b * ((g.N + b - 1) / b) + cus - 1) / cus) * b * b; };
-  if (rounds(256) < rounds(128) * TileSet<O>::kBigRate)
-    return launch_gemm_cfg<O, typename TileSet<O>::big, false>(g, e, 1, s, "loss_logits");
-  return launch_gemm_cfg<O, Tile<128, 128, 32, 2, 2>, false>(g, e, 1, s, "loss_logits");
+  auto time = [&](int64_t b, TileTime tt) {
+    return double(((g.M + b - 1) / b * ((g.N + b - 1) / b) + cus - 1) / cus) * (g.K / kPadK * tt.unit + tt.fixed);
+  };
+  if (time(256, tile_time<T, Big>()) <= time(128, tile_time<T, Small>()))
+    return launch_gemm_cfg<O, Big, false>(g, e, 1, s, "loss_logits");
+  return launch_gemm_cfg<O, Small, false>(g, e, 1, s, "loss_logits");
 }
 
 // dH and dW of a chunk from its S.
