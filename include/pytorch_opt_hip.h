@@ -283,7 +283,9 @@ int pto_shampoo_graft(void* p, const void* g, void* acc, const void* P, void* bu
  * dhidden and dweight, each if not NULL, from the forward call's norm and z.
  * The logits of at most about chunk_bytes (0: 2 GiB) are in the workspace at
  * any time: longer inputs go in chunks of rows. Sums are in a fixed order:
- * equal calls give equal bits.
+ * equal calls give equal bits. PTO_F32 products of more than 128 rows read each
+ * value as two fp16 numbers scaled by a power of two per row or column (an
+ * error of 2^-23 of the value or 2^-38 of the largest, whichever is more).
  */
 size_t pto_linear_loss_workspace_bytes(int dtype, int64_t rows, int64_t d, int64_t vocab, int64_t k, int64_t ldw,
                                        double label_smoothing, int distillation, int backward, int dhidden, int dweight, int64_t chunk_bytes);

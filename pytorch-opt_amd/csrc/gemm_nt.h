@@ -285,7 +285,7 @@ constexpr int kRowBytes = 64;
 
 __device__ __forceinline__ int swz(int r) { return ((r >> 2) & 3) ^ (r & 2); }
 
-// "QN" operand layout (bf16 only): Q is stored [K][N], N contiguous, the
+// "QN" operand layout (16-bit elements; fp32 at the end): Q is stored [K][N], N contiguous, the
 // natural layout of X in X' = B·X, so no transposed copy of X is needed.
 // A stage then holds BK rows of BN elements (BN*2 bytes) for Q, and the
 // MFMA B fragments come from transposing LDS reads (ds_read_b64_tr_b16).
@@ -307,6 +307,9 @@ __device__ __forceinline__ int swz(int r) { return ((r >> 2) & 3) ^ (r & 2); }
 //    only and so keeps every chunk inside its 128-byte group (below 24).
 // Both depend on row bits 0, 1 and 3 only, so the second half of a
 // fragment (4 rows on) keeps the swizzle.
+// fp32 rows, of a multiple of 256 bytes, are read a word per k: 16 lanes the
+// columns of row 4g + ii, the four groups' rows in two swizzles, so that two
+// of them share banks; the 16x16x4 MFMA takes 32 cycles and hides it.
 template <int RB>
 __device__ __forceinline__ int swzq(int r) {
   // (the kernel asserts RB % 256 is 0 or 128 wherever the layout is used)
@@ -722,8 +725,9 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_nt_kernel(Args g, Epi epi) {
   constexpr int PRB = PT ? BM * (int)sizeof(T) : kRowBytes;  // bytes per P row in LDS
   constexpr int CPRP = PRB / 16;                   // 16-byte chunks per P row
   static_assert((BM + BN) % (16 * NW) == 0 && IPW >= 1, "DMA split");
-  static_assert(!PT || (QN && CPRP >= 8 && (PRB % 256 == 0 || PRB % 256 == 128)),
-                "PT layout: with QN, P rows of 256·k or 256·k + 128 bytes");
+  constexpr bool kWords = std::is_same<T, float>::value;  // fp32 [K][·] operands: plain reads, a word per k
+  static_assert(!PT || (QN && CPRP >= 8 && (PRB % 256 == 0 || (!kWords && PRB % 256 == 128))),
+                "PT layout: with QN, P rows of 256·k or (16-bit elements) 256·k + 128 bytes");
   static_assert(WTM % MF::MN == 0 && WTN % MF::MN == 0 && WTM % 16 == 0, "wave tile");
   static_assert(KSPAN % VEC == 0 && NRG >= 1, "fragment runs");
   constexpr int NS = Cfg::NS;
@@ -735,9 +739,9 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_nt_kernel(Args g, Epi epi) {
   constexpr int KG = Cfg::KG, NWG = Cfg::WM * Cfg::WN;  // K groups, waves per group
   static_assert(KG == 1 || (FM % 2 == 0 && Plan::WTE % MF::MN == 0), "K groups: halves of whole fragments");
   static_assert(Cfg::NS * Plan::ARR <= Plan::kLdsMax, "LDS budget");
-  static_assert(!QN || (sizeof(T) == 2 && (!UPPER || PT) && CPR >= 8 && (QRB % 256 == 0 || QRB % 256 == 128) &&
-                        (BM * kRowBytes) % 1024 == 0 && NRG == 1),
-                "QN layout: bf16, Q rows of 256·k or 256·k + 128 bytes; symmetric products only with PT");
+  static_assert(!QN || ((sizeof(T) == 2 || (kWords && QRB % 256 == 0)) && (!UPPER || PT) && CPR >= 8 &&
+                        (QRB % 256 == 0 || QRB % 256 == 128) && (BM * kRowBytes) % 1024 == 0 && NRG == 1),
+                "QN layout: bf16 or fp32, Q rows of 256·k or 256·k + 128 bytes; symmetric products only with PT");
 
   // stages 4..7 exist (at full size) only in eight-stage rings
   constexpr int ARR_HI = NS > 4 ? Plan::ARR : 16;
@@ -903,7 +907,21 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_nt_kernel(Args g, Epi epi) {
   // second half (4 rows) add rows that keep the row's swizzle, which
   // depends on row bits 0, 1 and 3 only.
   int qoff[FN];
-  if constexpr (QN) {
+  // fp32: the word of column l % 16 in row KSPAN*lg; the next rows' swizzles
+  // (row bits 0 and 1) come on top of the offset
+  auto word_off = [&](int col, int rb) {
+    return KSPAN * lg * rb + (((col >> 2) ^ (8 * (lg >> 1))) << 4) + ((col & 3) << 2);
+  };
+  auto words = [&](const char* at, int off, int rb) {
+    unsigned w[4];
+#pragma unroll
+    for (int ii = 0; ii < 4; ++ii) w[ii] = *reinterpret_cast<const unsigned*>(at + ii * rb + (off ^ (ii << 5)));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  if constexpr (QN && kWords) {
+#pragma unroll
+    for (int fn = 0; fn < FN; ++fn) qoff[fn] = word_off(wn * WTN + fn * MF::MN + lr, QRB);
+  } else if constexpr (QN) {
     static_assert(KSPAN % 8 == 0, "QN row steps must keep the swizzle");
     const int li = lane & 15, qr = KSPAN * lg + (li >> 2);
 #pragma unroll
@@ -913,7 +931,10 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_nt_kernel(Args g, Epi epi) {
     }
   }
   int poff[FM];  // PT: the same for fragment fm of P (columns = rows of the output)
-  if constexpr (PT) {
+  if constexpr (PT && kWords) {
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm) poff[fm] = word_off(wm * WTM + fm * MF::MN + lr, PRB);
+  } else if constexpr (PT) {
     const int li = lane & 15, qr = KSPAN * lg + (li >> 2);
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
@@ -926,14 +947,17 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_nt_kernel(Args g, Epi epi) {
     uint4 a[NRG][FM], b[NRG][FN];
   };
   constexpr int kTileMfma = NRG * IPR * FM * FN;              // MFMAs per K tile
-  constexpr int kFragReads = NRG * ((PT ? 2 : 1) * FM + (QN ? 2 : 1) * FN);  // LDS reads per K tile
-  static_assert(kTileMfma % IPW == 0 && kFragReads % IPW == 0, "schedule groups");
+  constexpr int kRuns = kWords ? 4 : 2;  // reads of a [K][·] fragment
+  constexpr int kFragReads = NRG * ((PT ? kRuns : 1) * FM + (QN ? kRuns : 1) * FN);  // LDS reads per K tile
   // Order within a step: LDS reads for the next tile all first, or spread
   // between the MFMA groups (measured faster for the QN layout, slower for
   // the symmetric K-contiguous products).
   constexpr bool kSpreadReads = QN;
+  static_assert(kTileMfma % IPW == 0 && (!kSpreadReads || kFragReads % IPW == 0), "schedule groups");
   auto load_a = [&](const char* stage, int rg, int fm) -> uint4 {
-    if constexpr (PT) {
+    if constexpr (PT && kWords) {
+      return words(stage, poff[fm], PRB);
+    } else if constexpr (PT) {
       const char* Ps = stage + 8 * rg * PRB;
       v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(Ps + poff[fm]));
       v4i16_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(Ps + poff[fm] + 4 * PRB));
@@ -945,7 +969,9 @@ __global__ void __launch_bounds__(Cfg::NT) gemm_nt_kernel(Args g, Epi epi) {
     }
   };
   auto load_b = [&](const char* stage, int rg, int fn) -> uint4 {
-    if constexpr (QN) {
+    if constexpr (QN && kWords) {
+      return words(stage + BM * kRowBytes, qoff[fn], QRB);
+    } else if constexpr (QN) {
       // lanes of k-group lg, step rg: k = KSPAN*lg + 8*rg + 0..7
       const char* Qs = stage + BM * kRowBytes + 8 * rg * QRB;
       v4i16_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(Qs + qoff[fn]));

@@ -25,7 +25,9 @@
 //   dH, dW   two MFMA products (dW summed over the chunks in fp32).
 // A pass over V·rows logits is 2·rows·d·V operations, the three products
 // 6·rows·d·V: gradients found in the forward call need no second pass over the
-// logits (8·rows·d·V). Where the rows' gradients come later (losses per row),
+// logits (8·rows·d·V). bf16 runs on its own matrix instructions, fp32 on those
+// of fp16 (two planes per operand, three products; 2.9 times fp32's rate), and
+// where the rows are few on its own (few_rows). Where the rows' gradients come later (losses per row),
 // the normaliser and the targets' logits are kept and the backward call forms S
 // in the logits' epilogue.
 //
@@ -219,6 +221,13 @@ __global__ void __launch_bounds__(1024) list_rows_kernel(const int64_t* __restri
   }
 }
 
+// What the products read: bf16, fp32 as two fp16 planes (sp16), or, for few
+// rows, fp32 itself.
+template <class O>
+constexpr bool kPlanes = std::is_same<O, sp16>::value;
+template <class O>
+using Elem = std::conditional_t<kPlanes<O>, float, O>;
+
 // The rows of a chunk, as the kernels see them.
 struct Chunk {
   const int* list;
@@ -310,8 +319,16 @@ __global__ void __launch_bounds__(256) mark_targets_kernel(Chunk ch, int blocks,
 template <typename T>
 __device__ __forceinline__ void copy_row(const T* __restrict__ src, int64_t n, T* __restrict__ dst, int64_t ld,
                                          int lane) {
-  constexpr int E = 16 / (int)sizeof(T);
-  for (int64_t c = lane * E; c < ld; c += 64 * E) {
+  constexpr int E = 16 / (int)sizeof(T), STEP = 64 * E;
+  int64_t c = lane * E;
+  for (; c + 3 * STEP + E <= n; c += 4 * STEP) {  // loads in flight
+    uint4 u[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) u[q] = ld16(src + c + q * STEP);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(dst + c + q * STEP) = u[q];
+  }
+  for (; c < ld; c += STEP) {
     uint4 u = make_uint4(0, 0, 0, 0);
     if (c + E <= n) {
       u = ld16(src + c);
@@ -329,8 +346,9 @@ template <typename T>
 __device__ __forceinline__ void zero_row(T* __restrict__ row, int64_t d, int lane) {
   for (int64_t c = lane; c < d; c += 64) row[c] = T(0.f);
 }
-__global__ void __launch_bounds__(256) gather_kernel(Chunk ch, const bf16* __restrict__ h, int64_t ldh, int64_t d,
-                                                     bf16* __restrict__ hc, int64_t ldc, bf16* __restrict__ dh) {
+template <typename T>
+__global__ void __launch_bounds__(256) gather_kernel(Chunk ch, const T* __restrict__ h, int64_t ldh, int64_t d,
+                                                     T* __restrict__ hc, int64_t ldc, T* __restrict__ dh) {
   const int lane = threadIdx.x & 63;
   const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i < ch.live())
@@ -341,8 +359,9 @@ __global__ void __launch_bounds__(256) gather_kernel(Chunk ch, const bf16* __res
 }
 
 // W padded to a multiple of kPadK rows and columns.
-__global__ void __launch_bounds__(256) pad_weight_kernel(const bf16* __restrict__ w, int64_t ldw, int64_t vocab,
-                                                         int64_t d, bf16* __restrict__ out, int64_t ldo, int64_t rows) {
+template <typename T>
+__global__ void __launch_bounds__(256) pad_weight_kernel(const T* __restrict__ w, int64_t ldw, int64_t vocab,
+                                                         int64_t d, T* __restrict__ out, int64_t ldo, int64_t rows) {
   const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= rows) return;
   copy_row(w + min(r, vocab - 1) * ldw, r < vocab ? d : 0, out + r * ldo, ldo, threadIdx.x & 63);
@@ -350,8 +369,9 @@ __global__ void __launch_bounds__(256) pad_weight_kernel(const bf16* __restrict_
 
 // The rows of W from the last multiple of kPadK on, at W's pitch and with zero
 // rows up to the next (tail), and its last row by itself, padded to ldo.
-__global__ void __launch_bounds__(256) weight_tail_kernel(const bf16* __restrict__ w, int64_t ldw, int64_t vocab,
-                                                          int64_t d, bf16* __restrict__ tail, bf16* __restrict__ last,
+template <typename T>
+__global__ void __launch_bounds__(256) weight_tail_kernel(const T* __restrict__ w, int64_t ldw, int64_t vocab,
+                                                          int64_t d, T* __restrict__ tail, T* __restrict__ last,
                                                           int64_t ldo) {
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int64_t v = vocab / kPadK * kPadK + r;
@@ -408,7 +428,7 @@ __global__ void __launch_bounds__(256) weight_planes_kernel(const float* __restr
   const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r < vocab) row_planes(w + r * ldw, d, out + r * ld, vocab * ld, ld, exponent + r, nullptr, threadIdx.x & 63);
 }
-// gather_kernel for fp32: H as it is and as planes; also clears the maxima of
+// gather_kernel for planes: H as it is and as planes; also clears the maxima of
 // the chunk's columns.
 __global__ void __launch_bounds__(256) gather_planes_kernel(Chunk ch, const float* __restrict__ h, int64_t ldh,
                                                             int64_t d, float* __restrict__ hc, int64_t ldc,
@@ -467,10 +487,11 @@ struct RowSlope {
 // Epilogue of the logits' product, from the accumulators (kDirect): 16 lanes
 // have a row's 64 columns, four each. Through LDS staging in runs of eight the
 // same work took 14 us of a 256² tile's 69 at d = 2048, most of it VALU.
-// fp32 inputs come as split operands, with a power of two per row of each.
-template <typename T, bool KEEP, bool SLOPE>
+// Split operands come with a power of two per row of each.
+template <class O, bool KEEP, bool SLOPE>
 struct EpiLogits {
-  typedef float S;
+  typedef Elem<O> T;
+  typedef char S;  // the staging slice holds a row's targets and scales, no values
   static constexpr bool kDirect = true;
   Chunk ch;
   int vocab;
@@ -481,7 +502,7 @@ struct EpiLogits {
   void* kept;      // KEEP: the kept logits (uint16_t or float); SLOPE: S
   int64_t ld;
   const RowSlope* row;
-  const int *eh, *ew;  // fp32: the exponents of the rows of H and W
+  const int *eh, *ew;  // planes: the exponents of the rows of H and W
   Targets tg;
   int k;
   float* targets;  // [cap][k], null: the targets' logits t, by rank
@@ -492,7 +513,7 @@ struct EpiLogits {
     return row0 < g.M;
   }
   __device__ __forceinline__ int p_row(int i) const { return in_place ? ch.list[ch.base + i] : i; }
-  __device__ __forceinline__ const void* q_last() const { return sizeof(T) == 2 ? last : nullptr; }
+  __device__ __forceinline__ const void* q_last() const { return kPlanes<O> ? nullptr : last; }
   __device__ __forceinline__ int q_rows() const { return vocab; }
   __device__ __forceinline__ void finish(int) const {}
   template <class V, int FM, int FN>
@@ -532,7 +553,7 @@ struct EpiLogits {
         }
       }
     }
-    if (sizeof(T) == 4) {
+    if (kPlanes<O>) {
       for (int r = lane; r < R; r += 64) er[r] = eh[min(wr0 + r, g.M - 1)];
 #pragma unroll
       for (int k = 0; k < 4; ++k) ec[k] = ew[min(c0 + k, vocab - 1)];
@@ -545,7 +566,7 @@ struct EpiLogits {
     __builtin_amdgcn_wave_barrier();
     auto value = [&](int fm, int r, int k) {
       const float v = acc[fm][k][r];
-      return sizeof(T) == 4 ? ldexpf(v, -er[fm * 16 + sub + r] - ec[k]) : v;
+      return kPlanes<O> ? ldexpf(v, -er[fm * 16 + sub + r] - ec[k]) : v;
     };
     if (targets) {
 #pragma unroll
@@ -718,7 +739,7 @@ __device__ __forceinline__ RowSlope row_slope(const LossSpec& sp, float2 norm, f
 __device__ __forceinline__ float at_target(const RowSlope& rs, float a, float put, float z) {
   return fmaf(rs.pa, pow2(z - rs.m), fmaf(-a, put, rs.pu));
 }
-// fp32: S/a of a row, its a, and the largest |S/a| of every column, as bits.
+// Planes: S/a of a row, its a, and the largest |S/a| of every column, as bits.
 struct RowsOut {
   RowSlope* slope;
   float* a;
@@ -740,21 +761,23 @@ struct RowsOut {
 
 // Workgroups (y) per listed row, each with a run of its columns (few rows would
 // leave CUs idle): the normaliser, the loss and, for gradients
-// (SLOPES), S/alpha in place of the kept logits (bf16) or what the passes over
-// them need (fp32). losses is per row of the call; norm (m, s) and z (the
+// (SLOPES), S/alpha in place of the kept logits or what the passes over them
+// need (planes). losses is per row of the call; norm (m, s) and z (the
 // targets' logits in the caller's order) per listed row.
-template <typename T, bool SLOPES>
+template <class O, bool SLOPES>
 __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __restrict__ stats,
                                                      const float* __restrict__ sums, int64_t blocks, LossSpec sp,
                                                      Targets tg, const float* __restrict__ caught, int vocab,
-                                                     bf16* __restrict__ kept, int64_t ld, RowsOut out,
+                                                     Elem<O>* __restrict__ kept, int64_t ld, RowsOut out,
                                                      const float* __restrict__ alpha, float* __restrict__ losses,
                                                      float2* __restrict__ norms, float* __restrict__ z) {
+  typedef Elem<O> T;
+  constexpr int E = 16 / (int)sizeof(T);
   const int i = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t c0 = ld / kCols * blockIdx.y / gridDim.y * kCols, c1 = ld / kCols * (blockIdx.y + 1) / gridDim.y * kCols;
   if (i >= ch.live()) {
-    if (SLOPES && sizeof(T) == 2 && i < ch.padded())
-      for (int64_t c = c0 + tid * 8; c < c1; c += 2048) *reinterpret_cast<uint4*>(kept + i * ld + c) = make_uint4(0, 0, 0, 0);
+    if (SLOPES && !kPlanes<O> && i < ch.padded())
+      for (int64_t c = c0 + tid * E; c < c1; c += 256 * E) *reinterpret_cast<uint4*>(kept + i * ld + c) = make_uint4(0, 0, 0, 0);
     return;
   }
   const int row = ch.list[ch.base + i];
@@ -806,37 +829,44 @@ __global__ void __launch_bounds__(256) finish_kernel(Chunk ch, const float2* __r
     norms[ch.base + i] = norm;
   }
   if constexpr (SLOPES) {
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (kPlanes<O>) {
       out.put(i, sp, norm, qz, alpha[0], rt, zr, tid, 256);
       return;
     }
     const RowSlope rs = row_slope(sp, norm, qz, 1.f);
-    for (int64_t c = c0 + tid * 8; c < c1; c += 2048) {
+    for (int64_t c = c0 + tid * E; c < c1; c += 256 * E) {
       const uint4 u = *reinterpret_cast<const uint4*>(kept + i * ld + c);
       const unsigned uw[4] = {u.x, u.y, u.z, u.w};
       const float off = (st[c / kCols].x - m) - kOctaves;
-      float o[8];
+      float p[E], o[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const unsigned x = e & 1 ? uw[e / 2] >> 16 : uw[e / 2] & 0xffffu;
-        const float p = x ? pow2(fmaf((float)x, kOctaves / 65535.f, off)) : 0.f;
-        o[e] = c + e < vocab ? fmaf(rs.pa, p, rs.pu) : 0.f;
+      for (int e = 0; e < E; ++e) {
+        if constexpr (sizeof(T) == 4) {
+          p[e] = pow2(__uint_as_float(uw[e]) - m);
+        } else {
+          const unsigned x = e & 1 ? uw[e / 2] >> 16 : uw[e / 2] & 0xffffu;
+          p[e] = x ? pow2(fmaf((float)x, kOctaves / 65535.f, off)) : 0.f;
+        }
+        o[e] = c + e < vocab ? fmaf(rs.pa, p[e], rs.pu) : 0.f;
       }
-      st8<bf16, float>(kept + i * ld + c, o, 0, 8);
+      if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<float4*>(kept + i * ld + c) = make_float4(o[0], o[1], o[2], o[3]);
+      else
+        st8<bf16, float>(kept + i * ld + c, o, 0, 8);
     }
     __syncthreads();  // the dense part is written before the targets' entries replace theirs
     for (int e = tid; e < sp.k; e += 256) {
       const int id = rt.id(e);
       if (id >= c0 && id < c1 && rt.put(e) >= 0.f)
-        kept[i * ld + id] = bf16(at_target(rs, 1.f, rt.put(e), caught[tg.one ? i : (int64_t)i * sp.k + tg.rank[(int64_t)i * sp.k + e]]));
+        kept[i * ld + id] = T(at_target(rs, 1.f, rt.put(e), caught[tg.one ? i : (int64_t)i * sp.k + tg.rank[(int64_t)i * sp.k + e]]));
     }
   }
 }
 
 // Gradients of losses per row, normaliser and targets' logits kept: what the
-// logits' epilogue (bf16: S/alpha) or the passes over them (fp32) need of each
+// logits' epilogue (S/alpha) or the passes over them (planes) need of each
 // row; pad rows 0. One wave per row.
-template <typename T>
+template <class O>
 __global__ void __launch_bounds__(256) row_slopes_kernel(Chunk ch, LossSpec sp, Targets tg, const float* __restrict__ z,
                                                          const float2* __restrict__ norms,
                                                          const float* __restrict__ grad_rows, float scale,
@@ -856,21 +886,22 @@ __global__ void __launch_bounds__(256) row_slopes_kernel(Chunk ch, LossSpec sp, 
     if (rt.id(e) != -1) qz += rt.q(e) * (zr[e] - norm.x);
   qz = wave_sum(qz);
   const float a = grad_rows[row] * scale;
-  if constexpr (sizeof(T) == 4) {
+  if constexpr (kPlanes<O>) {
     out.put(i, sp, norm, qz, a, rt, zr, lane, 64);
   } else if (lane == 0) {
     out.slope[i] = row_slope(sp, norm, qz, a / alpha[0]);
     out.a[i] = a / alpha[0];
   }
 }
+template <typename T>
 __global__ void __launch_bounds__(64) put_targets_kernel(Chunk ch, int k, Targets tg, const float* __restrict__ z,
-                                                         RowsOut rows, bf16* __restrict__ s, int64_t ld) {
+                                                         RowsOut rows, T* __restrict__ s, int64_t ld) {
   const int i = blockIdx.x;
   if (i >= ch.live()) return;
   const int64_t at = ch.base + i;
   const RowTargets t{tg, at, ch.list[at], k};
   for (int e = threadIdx.x; e < k; e += 64)
-    if (t.id(e) >= 0 && t.put(e) >= 0.f) s[i * ld + t.id(e)] = bf16(at_target(rows.slope[i], rows.a[i], t.put(e), z[at * k + e]));
+    if (t.id(e) >= 0 && t.put(e) >= 0.f) s[i * ld + t.id(e)] = T(at_target(rows.slope[i], rows.a[i], t.put(e), z[at * k + e]));
 }
 
 // The loss of the call: a sum in a fixed order, over the count for the mean
@@ -893,7 +924,7 @@ __global__ void __launch_bounds__(1024) reduce_loss_kernel(const float* __restri
   if (threadIdx.x == 0) out[0] = (float)(red[0] / (mean ? max(1, count[0]) : 1));
 }
 
-// fp32: S/a and a·H as split planes for the gradients' products. dW sums over
+// S/a and a·H as split planes for the gradients' products. dW sums over
 // the rows, so a column of each has an exponent of its own, from its largest
 // value: tokens that are unlikely in every row keep their bits. dH sums over
 // the vocabulary, with the columns' exponents taken out of W's rows (undo); a,
@@ -1053,9 +1084,10 @@ struct EpiPlain {
 };
 
 // dH: rows of the chunk to their places, times what S is without: alpha, or
-// each row's a (fp32).
-template <typename T>
+// each row's a (planes).
+template <class O>
 struct EpiRows : EpiPlain {
+  typedef Elem<O> T;
   Chunk ch;
   T* dst;
   int64_t ld;
@@ -1065,7 +1097,7 @@ struct EpiRows : EpiPlain {
     return row0 < g.M;
   }
   __device__ __forceinline__ void put(int, int i, int j0, const S* v, int kbeg, int n, const Pre&, S*) const {
-    const float f = a[sizeof(T) == 4 ? i : 0];
+    const float f = a[kPlanes<O> ? i : 0];
     S w[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) w[k] = v[k] * f;
@@ -1074,9 +1106,11 @@ struct EpiRows : EpiPlain {
 };
 
 // dW over the chunks of rows: acc = v (first), acc + v, and out = acc + v,
-// times alpha (bf16) and rounded (last); acc is out where the chunk is the only one or out is fp32.
-template <typename T>
+// times alpha (S of planes is without each row's a, which H has) and rounded
+// (last); acc is out where the chunk is the only one or out is fp32.
+template <class O>
 struct EpiWeight : EpiPlain {
+  typedef Elem<O> T;
   Chunk ch;
   float* acc;
   T* out;
@@ -1085,7 +1119,8 @@ struct EpiWeight : EpiPlain {
   const float* alpha;
   typedef Raw8<float> Pre;
   __device__ __forceinline__ bool adjust(GemmArgs& g, int, int, int) const {
-    g.K = ch.padded();
+    // fp32: rows as far as its rings of K tiles (64)
+    g.K = std::is_same<O, float>::value ? (ch.live() + 63) / 64 * 64 : ch.padded();
     return g.K > 0 || first || last;
   }
   __device__ __forceinline__ void load(int, int i, int j0, int kbeg, int n, Pre& p) const {
@@ -1101,7 +1136,7 @@ struct EpiWeight : EpiPlain {
 #pragma unroll
       for (int k = 0; k < 8; ++k) r[k] += v[k];
     }
-    if (last && sizeof(T) == 2) {
+    if (last && !kPlanes<O>) {
       const float f = alpha[0];
 #pragma unroll
       for (int k = 0; k < 8; ++k) r[k] *= f;
@@ -1313,29 +1348,25 @@ struct Call {
   const char* name;
 };
 
-// Operand type of a dtype's products.
-template <typename T>
-using Operand = std::conditional_t<sizeof(T) == 4, sp16, bf16>;
-
-// Microseconds of a tile on one CU (128² tiles run in twos), measured.
-template <typename T, class Cfg>
+// Microseconds of a tile on one CU (the smaller run in twos), measured.
+template <class O, class Cfg>
 constexpr TileTime tile_time() {
-  constexpr bool big = Cfg::BM == 256;
-  return {(sizeof(T) == 4 ? 8.25f : 3.6f) / 65536 * Cfg::BM * Cfg::BN * (big ? 1.f : (float)TileSet<Operand<T>>::kBigRate),
-          sizeof(T) == 4 ? (big ? 20.f : 5.f) : (big ? 11.5f : 3.5f)};
+  constexpr bool big = Cfg::BM == TileSet<O>::big::BM;
+  constexpr float rate = std::is_same<O, float>::value ? 30.f : kPlanes<O> ? 8.25f : 3.6f;
+  return {rate / 65536 * Cfg::BM * Cfg::BN * (big ? 1.f : (float)TileSet<O>::kBigRate),
+          std::is_same<O, float>::value ? 4.f : kPlanes<O> ? (big ? 20.f : 5.f) : (big ? 11.5f : 3.5f)};
 }
 // From this many rounds of tiles on, the last one is not worth parts.
 constexpr int kWholeRounds = 12;
 constexpr int64_t kPartFloats = 2 * 65536;  // per CU: two rounds of partial 256² tiles
 
-template <typename T, class Cfg, class In, bool QN, bool PT, bool TAIL>
-int launch_gradient_cfg(const ArgsOf<Operand<T>>& args, const In& in, float* part, hipStream_t s, const char* name,
+template <class O, class Cfg, class In, bool QN, bool PT, bool TAIL>
+int launch_gradient_cfg(const ArgsOf<O>& args, const In& in, float* part, hipStream_t s, const char* name,
                     int tail_k, const void* tail) {
-  typedef Operand<T> O;
   typedef EpiSplit<In, Cfg, QN, PT, O, TAIL> Epi;
   ArgsOf<O> g = args;
-  PTO_REQUIRE(g.K % ring_k<O>() == 0 && g.ldq < (int64_t(1) << 26) && g.ldp < (int64_t(1) << 26) && g.ldp % 8 == 0 &&
-                  g.ldq % 8 == 0 && (!QN || g.ldq >= g.N) && (!PT || g.ldp >= g.M) &&
+  PTO_REQUIRE(g.K % ring_k<O>() == 0 && g.ldq < (int64_t(1) << 26) && g.ldp < (int64_t(1) << 26) && g.ldp * sizeof(O) % 16 == 0 &&
+                  g.ldq * sizeof(O) % 16 == 0 && (!QN || g.ldq >= g.N) && (!PT || g.ldp >= g.M) &&
                   ((reinterpret_cast<uintptr_t>(g.P) | reinterpret_cast<uintptr_t>(g.Q)) & 15) == 0,
               std::string(name) + ": operands not padded or not 16-byte aligned");
   g.tiles_m = (g.M + Cfg::BM - 1) / Cfg::BM;
@@ -1345,9 +1376,9 @@ int launch_gradient_cfg(const ArgsOf<Operand<T>>& args, const In& in, float* par
   if (tiles == 0) return 0;
   // dW's tiles are known here, and fewer rows make parts pay less
   const bool whole = tiles >= kWholeRounds * g.cus ||
-                     (PT && split_parts((int)tiles, g.K / kPadK, g.cus, tile_time<T, Cfg>(), Cfg::BM * Cfg::BN,
+                     (PT && split_parts((int)tiles, g.K / kPadK, g.cus, tile_time<O, Cfg>(), Cfg::BM * Cfg::BN,
                                         kMostParts).parts == 1);
-  Epi e{in, part, tile_time<T, Cfg>(), whole ? 1 : kMostParts, g.cus};
+  Epi e{in, part, tile_time<O, Cfg>(), whole ? 1 : kMostParts, g.cus};
   if (TAIL) {
     e.tail_k = tail_k;
     e.tail_bytes_ = static_cast<const char*>(tail) - static_cast<const char*>(g.Q) - (int64_t)tail_k * g.ldq * (int64_t)sizeof(O);
@@ -1366,28 +1397,32 @@ int launch_gradient_cfg(const ArgsOf<Operand<T>>& args, const In& in, float* par
   return 0;
 }
 // With the tile that ends sooner if every row counts.
-template <typename T, bool QN, bool PT, class In>
-int launch_gradient(const ArgsOf<Operand<T>>& g, const In& in, float* part, hipStream_t s, const char* name,
+template <class O, bool QN, bool PT, class In>
+int launch_gradient(const ArgsOf<O>& g, const In& in, float* part, hipStream_t s, const char* name,
                     int tail_k = 0, const void* tail = nullptr) {
-  typedef typename TileSet<Operand<T>>::big Big;
-  typedef typename TileSet<Operand<T>>::small Small;
+  // dW of few fp32 rows is mostly written, and five workgroups a CU write it 3%
+  // (3584 x 21675) to 5% (1024 x 32000) sooner than two of 128² tiles
+  if constexpr (std::is_same<O, float>::value && PT)
+    return launch_gradient_cfg<O, Tile<64, 64, 16, 2, 2>, In, QN, PT, false>(g, in, part, s, name, 0, nullptr);
+  typedef typename TileSet<O>::big Big;
+  typedef typename TileSet<O>::small Small;
   const int cus = device_cus(), units = g.K / kPadK;
   auto time = [&](int bm, int bn, TileTime tt) {
     const int tiles = ((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn);
     const Parts p = split_parts(tiles, units, cus, tt, bm * bn, kMostParts);
     return p.time + (float)(p.full / cus) * (units * tt.unit + tt.fixed);
   };
-  const bool big = time(Big::BM, Big::BN, tile_time<T, Big>()) <= time(Small::BM, Small::BN, tile_time<T, Small>());
-  if constexpr (QN && !PT && sizeof(T) == 2) {
+  const bool big = time(Big::BM, Big::BN, tile_time<O, Big>()) <= time(Small::BM, Small::BN, tile_time<O, Small>());
+  if constexpr (QN && !PT && !kPlanes<O>) {
     if (tail)
-      return big ? launch_gradient_cfg<T, Big, In, QN, PT, true>(g, in, part, s, name, tail_k, tail)
-                 : launch_gradient_cfg<T, Small, In, QN, PT, true>(g, in, part, s, name, tail_k, tail);
+      return big ? launch_gradient_cfg<O, Big, In, QN, PT, true>(g, in, part, s, name, tail_k, tail)
+                 : launch_gradient_cfg<O, Small, In, QN, PT, true>(g, in, part, s, name, tail_k, tail);
   }
-  return big ? launch_gradient_cfg<T, Big, In, QN, PT, false>(g, in, part, s, name, 0, nullptr)
-             : launch_gradient_cfg<T, Small, In, QN, PT, false>(g, in, part, s, name, 0, nullptr);
+  return big ? launch_gradient_cfg<O, Big, In, QN, PT, false>(g, in, part, s, name, 0, nullptr)
+             : launch_gradient_cfg<O, Small, In, QN, PT, false>(g, in, part, s, name, 0, nullptr);
 }
 
-// Whether bf16 products read W where it lies, else from a padded copy. They can
+// Whether the products (not of planes) read W where it lies, else from a padded copy. They can
 // where its rows are 16-byte aligned and what follows a row's end up to a
 // multiple of kPadK is nothing but the next row (an infinity there times H's
 // zero makes a NaN of a row that it would have made infinite itself), and do
@@ -1396,27 +1431,28 @@ int launch_gradient(const ArgsOf<Operand<T>>& g, const In& in, float* part, hipS
 // rows that are no whole 128-byte lines 50, a tail of the vocabulary 5% of dH
 // (8192 x 2048 x 32000: 15 against 53 for the copy, 64 x 2240 x 35072: 2
 // against 52).
-inline bool reads_in_place(const Call& c, int64_t dp) {
-  if (c.ldw % 8 || (c.d % kPadK && (c.ldw != c.d || dp - c.d > c.d))) return false;
-  return (c.d % kPadK == 0 && (!c.dh || c.vocab % kPadK == 0)) || c.rows <= (c.ldw % 64 ? 1024 : 8192);
+inline bool reads_in_place(const Call& c, int64_t dp, int64_t element) {
+  if (c.ldw * element % 16 || (c.d % kPadK && (c.ldw != c.d || dp - c.d > c.d))) return false;
+  return (c.d % kPadK == 0 && (!c.dh || c.vocab % kPadK == 0)) || c.rows <= (c.ldw * element % 128 ? 1024 : 8192);
 }
 
-template <typename T>
+template <class O>
 struct Ws {
-  static constexpr bool f32 = sizeof(T) == 4;
+  typedef Elem<O> T;
+  static constexpr bool planes = kPlanes<O>;
   int64_t dp, vp, blocks, cap, capp;
   bool pad_w, in_place;
   Targets t{};
   int *list, *count;
   T* hc;
-  // bf16: W padded; or its last rows up to a multiple of kPadK and, by itself,
+  // W padded; or its last rows up to a multiple of kPadK and, by itself,
   // its last one
-  bf16 *wp, *tail, *last;
+  T *wp, *tail, *last;
   float2 *stats, *norm;
   float *sums, *losses, *z, *caught, *alpha;
   RowsOut rows;
-  T* kept;  // the kept logits, bf16: then S
-  // fp32: planes of H and W (by rows) for the logits, of S/a, W (S's exponents
+  T* kept;  // the kept logits; not of planes: then S
+  // Planes of H and W (by rows) for the logits, of S/a, W (S's exponents
   // taken out) and a·H (by columns) for the gradients
   sp16 *hp, *wpl, *sp, *ws, *ah;
   int *eh, *ew, *es, *ews, *eah;  // es, ews and eah: exponents of the columns' maxima
@@ -1428,11 +1464,11 @@ struct Ws {
     dp = round_up(c.d, kPadK);
     vp = round_up(c.vocab, kPadK);
     blocks = vp / kCols;
-    const int64_t per = grads ? vp * (f32 ? 8 : 2) : blocks * 8;
+    const int64_t per = grads ? vp * (planes ? 8 : (int64_t)sizeof(T)) : blocks * 8;
     cap = (c.chunk_bytes > 0 ? c.chunk_bytes : kChunkBytes) / per;
     cap = std::min(std::max<int64_t>(cap / 256 * 256, 256), std::max<int64_t>(c.rows, 1));
     capp = round_up(cap, kPadK);
-    pad_w = !f32 && !reads_in_place(c, dp);
+    pad_w = !planes && !reads_in_place(c, dp, sizeof(T));
     const bool join = !c.grad_rows;
     if (c.kd) {
       t.id = cv.take<int>(c.rows * c.k);
@@ -1453,30 +1489,30 @@ struct Ws {
     count = cv.take<int>(4);
     alpha = cv.take<float>(4);
     // scoring reads aligned rows of H where they lie
-    in_place = !f32 && !grads && c.h && c.d % kPadK == 0 && c.ldh % 8 == 0 && (reinterpret_cast<uintptr_t>(c.h) & 15) == 0;
+    in_place = !planes && !grads && c.h && c.d % kPadK == 0 && c.ldh * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(c.h) & 15) == 0;
     hc = in_place ? nullptr : cv.take<T>(capp * dp);
-    wp = pad_w ? cv.take<bf16>(vp * dp) : nullptr;
-    tail = !f32 && !pad_w && c.dh && c.vocab % kPadK ? cv.take<bf16>(kPadK * c.ldw) : nullptr;
-    last = !f32 && !pad_w && c.d % kPadK ? cv.take<bf16>(dp) : nullptr;
+    wp = pad_w ? cv.take<T>(vp * dp) : nullptr;
+    tail = !planes && !pad_w && c.dh && c.vocab % kPadK ? cv.take<T>(kPadK * c.ldw) : nullptr;
+    last = !planes && !pad_w && c.d % kPadK ? cv.take<T>(dp) : nullptr;
     losses = cv.take<float>(c.rows);
     norm = cv.take<float2>(c.rows);
     z = cv.take<float>(c.rows * c.k);
     caught = join ? cv.take<float>(cap * c.k) : nullptr;
-    stats = join || f32 ? cv.take<float2>(cap * blocks) : nullptr;
+    stats = join || planes ? cv.take<float2>(cap * blocks) : nullptr;
     sums = c.smooth != 0 && join ? cv.take<float>(cap * blocks) : nullptr;
-    rows = RowsOut{grads && (f32 || c.grad_rows) ? cv.take<RowSlope>(capp) : nullptr,
-                   grads && (f32 || c.grad_rows) ? cv.take<float>(capp) : nullptr, nullptr};
+    rows = RowsOut{grads && (planes || c.grad_rows) ? cv.take<RowSlope>(capp) : nullptr,
+                   grads && (planes || c.grad_rows) ? cv.take<float>(capp) : nullptr, nullptr};
     kept = grads ? cv.take<T>(capp * vp) : nullptr;
     hp = wpl = sp = ws = ah = nullptr;
     eh = ew = es = ews = eah = nullptr;
     undo = parts = nullptr;
-    if (f32) {
+    if (planes) {
       hp = cv.take<sp16>(2 * capp * dp);
       wpl = cv.take<sp16>(2 * c.vocab * dp);
       eh = cv.take<int>(capp);
       ew = cv.take<int>(c.vocab);
     }
-    if (f32 && grads) {
+    if (planes && grads) {
       rows.maxima = cv.take<unsigned>(vp);
       es = cv.take<int>(vp + 2 * dp);
       eah = es + vp;
@@ -1490,15 +1526,25 @@ struct Ws {
       }
     }
     part = grads ? cv.take<float>(kPartFloats * device_cus()) : nullptr;
-    acc = !f32 && c.dw && chunks(c) > 1 ? cv.take<float>(c.vocab * c.d) : nullptr;
+    acc = sizeof(T) == 2 && c.dw && chunks(c) > 1 ? cv.take<float>(c.vocab * c.d) : nullptr;
   }
 };
 
-template <typename T>
+template <class O>
 size_t loss_ws_bytes(const Call& c) {
   Carver cv(nullptr, 0);
-  Ws<T> w(cv, c);
+  Ws<O> w(cv, c);
   return cv.used + 512;
+}
+
+// Whether fp32 products run on fp32's own matrix instructions, a third of the
+// planes' rate, but W read where it lies, where the planes take five passes over
+// it. Losses and gradients of 64 x 3584 x 21675 take 415 us (planes: 838), 128 x
+// 1024 x 32000 283 (412); at 192 rows one or the other is 13% faster by shape,
+// at 256 the planes by up to 20%. A padded copy of W costs scores as much as
+// their planes.
+inline bool few_rows(const Call& c) {
+  return c.rows <= kPadK && (c.dh || c.dw || reads_in_place(c, round_up(c.d, kPadK), 4));
 }
 
 // Workgroups per row of `cols`: two per CU in all, 2048 columns each at least.
@@ -1506,40 +1552,42 @@ inline unsigned segments(int64_t rows, int64_t cols) {
   return (unsigned)std::max<int64_t>(1, std::min<int64_t>(2 * device_cus() / rows, cols / 2048));
 }
 
-// The logits' product: 256² or 128² tiles, both of 64-column wave tiles.
-template <typename T, class Epi>
-int launch_logits(const ArgsOf<Operand<T>>& g, const Epi& e, hipStream_t s) {
-  typedef Operand<T> O;
+// The logits' product: two sizes of tile, both of 64-column wave tiles.
+template <class O, class Epi>
+int launch_logits(const ArgsOf<O>& g, const Epi& e, hipStream_t s) {
   typedef typename TileSet<O>::big Big;
-  typedef Tile<128, 128, 32, 2, 2> Small;
+  typedef std::conditional_t<std::is_same<O, float>::value, Tile<64, 64, 16, 4, 1, 8>, Tile<128, 128, 32, 2, 2>> Small;
   const int64_t cus = device_cus();
   auto time = [&](int64_t b, TileTime tt) {
     return double(((g.M + b - 1) / b * ((g.N + b - 1) / b) + cus - 1) / cus) * (g.K / kPadK * tt.unit + tt.fixed);
   };
-  if (time(256, tile_time<T, Big>()) <= time(128, tile_time<T, Small>()))
+  if (time(Big::BM, tile_time<O, Big>()) <= time(Small::BM, tile_time<O, Small>()))
     return launch_gemm_cfg<O, Big, false>(g, e, 1, s, "loss_logits");
   return launch_gemm_cfg<O, Small, false>(g, e, 1, s, "loss_logits");
 }
 
 // dH and dW of a chunk from its S.
-int chunk_gradients(const Call& c, const Ws<bf16>& w, const Chunk& ch, const bf16* W, int64_t ldw, bool first, bool last,
+template <class O>
+int chunk_gradients(const Call& c, const Ws<O>& w, const Chunk& ch, const O* W, int64_t ldw, bool first, bool last,
                     hipStream_t s) {
   if (c.dh && ch.cap > 0) {
     const GemmArgs g{w.kept, w.vp, 0, W, ldw, 0, ch.cap, (int)c.d, (int)w.vp, 0, 0, nullptr};
-    const EpiRows<bf16> e{{}, ch, static_cast<bf16*>(c.dh), c.d, w.alpha};
-    if (launch_gradient<bf16, true, false>(g, e, w.part, s, "loss_dhidden", (int)(c.vocab / kPadK * kPadK), w.tail))
+    const EpiRows<O> e{{}, ch, static_cast<O*>(c.dh), c.d, w.alpha};
+    if (launch_gradient<O, true, false>(g, e, w.part, s, "loss_dhidden", (int)(c.vocab / kPadK * kPadK), w.tail))
       return -1;
   }
   if (c.dw) {
     const int k = (int)round_up(ch.cap, kPadK);
     const GemmArgs g{w.kept, w.vp, 0, w.hc, w.dp, 0, (int)c.vocab, (int)c.d, k, 0, 0, nullptr};
-    const EpiWeight<bf16> e{{}, ch, w.acc, static_cast<bf16*>(c.dw), c.d, first, last, w.alpha};
-    if (launch_gradient<bf16, true, true>(g, e, w.part, s, "loss_dweight")) return -1;
+    float* acc = w.acc;
+    if constexpr (sizeof(O) == 4) acc = static_cast<float*>(c.dw);
+    const EpiWeight<O> e{{}, ch, acc, static_cast<O*>(c.dw), c.d, first, last, w.alpha};
+    if (launch_gradient<O, true, true>(g, e, w.part, s, "loss_dweight")) return -1;
   }
   return 0;
 }
 
-int chunk_gradients(const Call& c, const Ws<float>& w, const Chunk& ch, const LossSpec& sp, const float* z, bool first,
+int chunk_gradients(const Call& c, const Ws<sp16>& w, const Chunk& ch, const LossSpec& sp, const float* z, bool first,
                     bool last, hipStream_t s) {
   float *dh = static_cast<float*>(c.dh), *dw = static_cast<float*>(c.dw);
   const int k = (int)round_up(ch.cap, kPadK), cap = ch.cap, vocab = (int)c.vocab, d = (int)c.d;
@@ -1573,8 +1621,8 @@ int chunk_gradients(const Call& c, const Ws<float>& w, const Chunk& ch, const Lo
                        w.rows.slope, w.undo, w.ews, w.ws, w.dp, w.vp * w.dp, sp.k, w.t, z);
     PTO_LAUNCHED("column_planes");
     const SplitArgs g{{w.sp, w.vp, 0, w.ws, w.dp, 0, cap, d, (int)w.vp}, w.capp * w.vp, w.vp * w.dp};
-    const EpiPowers<EpiRows<float>> e{{}, {{}, ch, dh, c.d, w.rows.a}, nullptr, w.ews, 0};
-    if (launch_gradient<float, true, false>(g, e, w.part, s, "loss_dhidden")) return -1;
+    const EpiPowers<EpiRows<sp16>> e{{}, {{}, ch, dh, c.d, w.rows.a}, nullptr, w.ews, 0};
+    if (launch_gradient<sp16, true, false>(g, e, w.part, s, "loss_dhidden")) return -1;
   }
   if (dw) {
     if (cap > 0) {
@@ -1583,17 +1631,18 @@ int chunk_gradients(const Call& c, const Ws<float>& w, const Chunk& ch, const Lo
       PTO_LAUNCHED("column_planes");
     }
     const SplitArgs g{{w.sp, w.vp, 0, w.ah, w.dp, 0, vocab, d, k}, w.capp * w.vp, w.capp * w.dp};
-    const EpiPowers<EpiWeight<float>> e{{}, {{}, ch, dw, dw, c.d, first, last, nullptr}, w.es, w.eah, 0};
-    if (launch_gradient<float, true, true>(g, e, w.part, s, "loss_dweight")) return -1;
+    const EpiPowers<EpiWeight<sp16>> e{{}, {{}, ch, dw, dw, c.d, first, last, nullptr}, w.es, w.eah, 0};
+    if (launch_gradient<sp16, true, true>(g, e, w.part, s, "loss_dweight")) return -1;
   }
   return 0;
 }
 
-template <typename T>
+template <class O>
 int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
-  constexpr bool f32 = sizeof(T) == 4;
+  typedef Elem<O> T;
+  constexpr bool planes = kPlanes<O>;
   Carver cv(ws, ws_bytes);
-  const Ws<T> w(cv, c);
+  const Ws<O> w(cv, c);
   PTO_REQUIRE(!cv.overflow, std::string(c.name) + ": workspace too small");
   const bool grads = c.dh || c.dw;
   const T* W = static_cast<const T*>(c.w);
@@ -1613,18 +1662,18 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
                      w.alpha);
   PTO_LAUNCHED("list_rows");
   if (c.rows > 0) {
-    if constexpr (f32) {
+    if constexpr (planes) {
       hipLaunchKernelGGL(weight_planes_kernel, dim3((unsigned)((c.vocab + 3) / 4)), dim3(256), 0, s, W, ldw, c.vocab,
                          c.d, w.wpl, w.dp, w.ew);
       PTO_LAUNCHED("weight_planes");
     } else if (w.pad_w) {
-      hipLaunchKernelGGL(pad_weight_kernel, dim3((unsigned)((w.vp + 3) / 4)), dim3(256), 0, s, W, ldw, c.vocab, c.d,
+      hipLaunchKernelGGL(pad_weight_kernel<T>, dim3((unsigned)((w.vp + 3) / 4)), dim3(256), 0, s, W, ldw, c.vocab, c.d,
                          w.wp, w.dp, w.vp);
       PTO_LAUNCHED("pad_weight");
       W = w.wp;
       ldw = w.dp;
     } else if (w.tail || w.last) {
-      hipLaunchKernelGGL(weight_tail_kernel, dim3(kPadK / 4), dim3(256), 0, s, W, ldw, c.vocab, c.d, w.tail, w.last, w.dp);
+      hipLaunchKernelGGL(weight_tail_kernel<T>, dim3(kPadK / 4), dim3(256), 0, s, W, ldw, c.vocab, c.d, w.tail, w.last, w.dp);
       PTO_LAUNCHED("weight_tail");
     }
   }
@@ -1634,8 +1683,8 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
     if (ch.cap > 0) {
       const unsigned capp = (unsigned)round_up(ch.cap, kPadK);
       GemmArgs base{w.hc, w.dp, 0, W, ldw, 0, ch.cap, (int)w.vp, (int)w.dp, 0, 0, nullptr};
-      ArgsOf<Operand<T>> g{base};
-      if constexpr (f32) {
+      ArgsOf<O> g{base};
+      if constexpr (planes) {
         hipLaunchKernelGGL(gather_planes_kernel, dim3(capp / 4), dim3(256), 0, s, ch, static_cast<const float*>(c.h),
                            c.ldh, c.d, w.hc, w.dp, w.hp, w.capp * w.dp, w.eh, static_cast<float*>(c.dh), w.rows.maxima,
                            grads ? w.vp : 0);
@@ -1648,8 +1697,8 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
         g.P = c.h;
         g.ldp = c.ldh;
       } else {
-        hipLaunchKernelGGL(gather_kernel, dim3(capp / 4), dim3(256), 0, s, ch, static_cast<const bf16*>(c.h), c.ldh,
-                           c.d, w.hc, w.dp, static_cast<bf16*>(c.dh));
+        hipLaunchKernelGGL(gather_kernel<T>, dim3(capp / 4), dim3(256), 0, s, ch, static_cast<const T*>(c.h), c.ldh,
+                           c.d, w.hc, w.dp, static_cast<T*>(c.dh));
       }
       PTO_LAUNCHED("gather");
       if (c.kd) {
@@ -1660,41 +1709,41 @@ int loss_t(const Call& c, void* ws, size_t ws_bytes, hipStream_t s) {
         PTO_LAUNCHED("mark_targets");
       }
       if (c.grad_rows) {
-        hipLaunchKernelGGL(row_slopes_kernel<T>, dim3(capp / 4), dim3(256), 0, s, ch, sp, w.t, z, norm, c.grad_rows,
+        hipLaunchKernelGGL(row_slopes_kernel<O>, dim3(capp / 4), dim3(256), 0, s, ch, sp, w.t, z, norm, c.grad_rows,
                            (float)c.temp, w.alpha, w.rows);
         PTO_LAUNCHED("row_slopes");
-        if constexpr (f32) {
-          const EpiLogits<T, true, false> e{ch,      (int)c.vocab, scale, w.stats, nullptr, w.blocks, w.kept,
+        if constexpr (planes) {
+          const EpiLogits<O, true, false> e{ch,      (int)c.vocab, scale, w.stats, nullptr, w.blocks, w.kept,
                                             w.vp,    nullptr,      w.eh,  w.ew,    w.t,     sp.k,     nullptr, false,
                                             w.last};
-          if (launch_logits<T>(g, e, s)) return -1;
+          if (launch_logits<O>(g, e, s)) return -1;
         } else {
           g.M = (int)capp;
-          const EpiLogits<T, false, true> e{ch,   (int)c.vocab, scale,   nullptr, nullptr, w.blocks, w.kept,
+          const EpiLogits<O, false, true> e{ch,   (int)c.vocab, scale,   nullptr, nullptr, w.blocks, w.kept,
                                             w.vp, w.rows.slope, nullptr, nullptr, w.t,     sp.k,     nullptr, false,
                                             w.last};
-          if (launch_logits<T>(g, e, s)) return -1;
-          hipLaunchKernelGGL(put_targets_kernel, dim3((unsigned)ch.cap), dim3(64), 0, s, ch, sp.k, w.t, z, w.rows,
+          if (launch_logits<O>(g, e, s)) return -1;
+          hipLaunchKernelGGL(put_targets_kernel<T>, dim3((unsigned)ch.cap), dim3(64), 0, s, ch, sp.k, w.t, z, w.rows,
                              w.kept, w.vp);
           PTO_LAUNCHED("put_targets");
         }
       } else {
         auto logits = [&](auto keep) {
-          const EpiLogits<T, decltype(keep)::value, false> e{ch,     (int)c.vocab, scale, w.stats, w.sums,
+          const EpiLogits<O, decltype(keep)::value, false> e{ch,     (int)c.vocab, scale, w.stats, w.sums,
                                                              w.blocks, w.kept,     w.vp,  nullptr, w.eh,
                                                              w.ew,   w.t,          sp.k,  w.caught, w.in_place,
                                                              w.last};
-          return launch_logits<T>(g, e, s);
+          return launch_logits<O>(g, e, s);
         };
         if (grads ? logits(std::true_type{}) : logits(std::false_type{})) return -1;
-        hipLaunchKernelGGL((grads ? finish_kernel<T, true> : finish_kernel<T, false>), dim3(capp, grads && !f32 ? segments(capp, w.vp) : 1), dim3(256), 0, s, ch,
-                           w.stats, w.sums, w.blocks, sp, w.t, w.caught, (int)c.vocab, reinterpret_cast<bf16*>(w.kept),
+        hipLaunchKernelGGL((grads ? finish_kernel<O, true> : finish_kernel<O, false>), dim3(capp, grads && !planes ? segments(capp, w.vp) : 1), dim3(256), 0, s, ch,
+                           w.stats, w.sums, w.blocks, sp, w.t, w.caught, (int)c.vocab, w.kept,
                            w.vp, w.rows, w.alpha, losses, norm, z);
         PTO_LAUNCHED("finish");
       }
     }
     const bool first = n == 0, last = n == chunks - 1;
-    if constexpr (f32) {
+    if constexpr (planes) {
       if (grads && chunk_gradients(c, w, ch, sp, z, first, last, s)) return -1;
     } else {
       if (grads && chunk_gradients(c, w, ch, W, ldw, first, last, s)) return -1;
@@ -1734,7 +1783,8 @@ int check(const Call& c, int dtype, void* ws, size_t ws_bytes) {
 int run(const Call& c, int dtype, void* ws, size_t ws_bytes, void* stream) {
   if (check(c, dtype, ws, ws_bytes)) return -2;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == kBF16 ? loss_t<bf16>(c, ws, ws_bytes, s) : loss_t<float>(c, ws, ws_bytes, s);
+  if (dtype == kBF16) return loss_t<bf16>(c, ws, ws_bytes, s);
+  return few_rows(c) ? loss_t<float>(c, ws, ws_bytes, s) : loss_t<sp16>(c, ws, ws_bytes, s);
 }
 
 }  // namespace
@@ -1762,7 +1812,7 @@ size_t pto_linear_loss_workspace_bytes(int dtype, int64_t rows, int64_t d, int64
   c.chunk_bytes = chunk_bytes;
   switch (dtype) {
     case pto::kBF16: return pto::loss_ws_bytes<pto::bf16>(c);
-    case pto::kF32: return pto::loss_ws_bytes<float>(c);
+    case pto::kF32: return pto::few_rows(c) ? pto::loss_ws_bytes<float>(c) : pto::loss_ws_bytes<pto::sp16>(c);
     default: return 0;
   }
 }

@@ -326,6 +326,55 @@ def test_wide_logits(native_backend, dtype):
     _check(_exact_ce(h.detach(), w.detach(), y, reduction="sum"), loss.detach(), dh, dw, dtype, "sum")
 
 
+def _plane_floor(e):
+    """What fp16 planes add to the bounds on (dH, dW), whatever a value's own
+    size: fp16 holds multiples of 2^-24, so a plane of a column scaled to a
+    maximum of at least 2^13 is off by up to 2^-25·2^-13 of that maximum. dW
+    sums S/a by columns against a·H by columns, dH S/a against W's rows times
+    the maxima of S/a."""
+    a = torch.where(e.a == 0, 1.0, e.a)
+    s, ah = (e.S / a).abs(), (e.a * e.h).abs()
+    top = s.amax(0)
+    floor = 2.0 ** -38
+    dw = floor * (top[:, None] * ah.sum(0) + s.sum(0)[:, None] * ah.amax(0))
+    scaled = top[:, None] * e.w.abs()
+    dh = floor * e.a.abs() * (scaled.sum(0) + (s / top.clamp_min(1e-300)).sum(1, keepdim=True) * scaled.amax(0))
+    return dh, dw
+
+
+# fp32 products take another form from 129 rows on
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [16, 65, 128, 129, 180])
+@pytest.mark.parametrize("d,vocab", [(72, 515), (610, 1100), (256, 1500)])
+def test_few_rows_and_more_in_float32(native_backend, rows, d, vocab):
+    """Wide logits, equal ids, left-out rows that hold anything, an unaligned
+    weight whose neighbours are not numbers."""
+    h, w, g = _make(rows, d, vocab, torch.float32, seed=rows + d, scale=20.0)
+    pool = torch.full((w.numel() + 9,), float("nan"), device=DEV)
+    w = pool[5:5 + w.numel()].view_as(w).copy_(w).requires_grad_()
+    index = torch.randint(0, 40, (rows, 70), generator=g).to(DEV)
+    logits = torch.randn(rows, 70, generator=g).to(DEV)
+    y = _targets(rows, vocab, g, 0.7)
+    gone = y == IGNORE
+    index[gone] = -1
+    h[gone] = float("nan")
+    h.requires_grad_()
+    clean = torch.where(gone[:, None], 0.0, h.detach())
+    for reduction in ("mean", "none"):
+        weights = torch.randn(rows, generator=g).to(DEV) if reduction == "none" else None
+        g_rows = None if weights is None else weights.double()
+        for loss, e in ((ops.linear_cross_entropy(h, w, y, reduction=reduction),
+                         _exact_ce(clean, w.detach(), y, 0.0, 0.0, g_rows, reduction)),
+                        (ops.linear_distillation(h, w, logits, index, temperature=1.5, reduction=reduction),
+                         _exact_kd(clean, w.detach(), logits, index, 1.5, g_rows, reduction))):
+            dh, dw = torch.autograd.grad(loss, (h, w), weights)
+            if rows > 128:
+                bl, bh, bw = e.bounds(torch.float32)
+                fh, fw = _plane_floor(e)
+                e.bounds = lambda dtype: (bl, bh + fh, bw + fw)
+            _check(e, loss.detach(), dh, dw, torch.float32, reduction)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_target_outside_the_vocabulary_is_nan(native_backend, dtype):
