@@ -1554,11 +1554,11 @@ size_t loss_ws_bytes(const Call& c) {
 }
 
 // Whether fp32 products run on fp32's own matrix instructions, a third of the
-// planes' rate, but W read where it lies, where the planes take five passes over
-// it. Losses and gradients of 64 x 3584 x 21675 take 415 us (planes: 838), 128 x
-// 1024 x 32000 283 (412); at 192 rows one or the other is 13% faster by shape,
-// at 256 the planes by up to 20%. A padded copy of W costs scores as much as
-// their planes.
+// planes' rate, but W's bytes are read twice, where the planes read or write
+// them seven times. Losses and gradients of 64 x 3584 x 21675 take 415 us
+// (planes: 838), 128 x 1024 x 32000 283 (412); at 192 rows one or the other is
+// 13% faster by shape, at 256 the planes by up to 20%. A padded copy of W costs
+// scores as much as their planes.
 inline bool few_rows(const Call& c) {
   return c.rows <= kPadK && (c.dh || c.dw || reads_in_place(c, round_up(c.d, kPadK), 4));
 }
